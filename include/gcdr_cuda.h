@@ -289,8 +289,9 @@ typedef struct {
  * read by gcdr_k_status. */
 GCDR_API int gcdr_k_conv(const gcdr_conv_desc *d, int reference, void *stream);
 /* Waits for `stream`, then reads and clears the current device's layer error
- * word: GCDR_ERR_TIMEOUT if a gcdr_k_conv kernel gave up on a wait since the
- * last gcdr_k_status, else GCDR_OK (GCDR_ERR_DEVICE if the stream failed). */
+ * word: GCDR_ERR_TIMEOUT if a gcdr_k_conv or gcdr_k_i8_gemm kernel gave up on a
+ * wait since the last gcdr_k_status, else GCDR_OK (GCDR_ERR_DEVICE if the stream
+ * failed). */
 GCDR_API int gcdr_k_status(void *stream);
 /* Repacks fp16 NHWC [H][W][C] into a layer input layout:
  *   kind 1  [H+2][W+2][C] with a reflect border
@@ -359,6 +360,100 @@ GCDR_API int gcdr_device_sms(void);
  *   - One workspace per device: calls that overlap in time race on it. */
 #define GCDR_STATIC_WS_BYTES (16 * 1024 * 1024)
 GCDR_API int gcdr_k_conv_static(const gcdr_conv_desc *d, void *stream);
+
+/* ------------------------------------------------- 8-bit token operators
+ *
+ * The token products of an int8 deployment and what surrounds them, beside the fp16 token
+ * Gemm (gcdr_k_conv kind 2) and its LayerNorm finalize.  No counterpart in the reference (its
+ * engines run fp32).  A chain of them, as one block uses it:
+ *
+ *   gcdr_k_block_norm  (norm; rows out as int8)  ->  gcdr_k_i8_gemm  ->  gcdr_k_dw_gelu_shift
+ *   ->  gcdr_k_quant_rows  ->  gcdr_k_i8_gemm  ->  gcdr_k_block_norm  (post-norm, gate, residual)
+ *
+ * Common to the three.  All pointers are DEVICE pointers of the current device (anything
+ * else is GCDR_ERR_ARG); calls only enqueue work on `stream` (NULL = default stream), allocate
+ * nothing, and may be captured into a graph.  Rows lie `ld` elements apart (ld >= the row's length);
+ * what lies between a row's end and the next row is neither read nor written.  An output may not overlap
+ * another operand, except that r and y of gcdr_k_block_norm may be x or f itself at the same pitch.  Zero
+ * rows: GCDR_OK, nothing is launched.  A refused call prints the reason to stderr and launches
+ * nothing: GCDR_ERR_ARG (null, unaligned, overlapping or foreign operands, unknown codes), GCDR_ERR_RANGE
+ * (sizes and pitches).  Results do not depend on the launch: the same inputs give the same bytes. */
+#define GCDR_DTYPE_F16 0
+#define GCDR_DTYPE_BF16 1
+#define GCDR_DTYPE_F32 2
+#define GCDR_NORM_NONE 0
+#define GCDR_NORM_LAYER 1
+#define GCDR_NORM_RMS 2
+
+/* Rows to int8 with a scale each: scale = max|x| / 127 (fp32), q = x * 127 / max|x| to nearest even
+ * (exact for every input), so q * scale stands for x.  For tokens, and for weights [N][K] (a scale for
+ * each output channel).  x: rows x C of `dtype`, C 1..32768.  A row of zeros: scale 0, q 0.  A row
+ * that holds an infinity or NaN: scale NaN, q 0 (its products are NaN). */
+GCDR_API int gcdr_k_quant_rows(const void *x, int dtype, int64_t rows, int C, int64_t ldx, int8_t *q,
+                               int64_t ldq, float *scale, void *stream);
+
+/* out[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], then relu (a NaN stays NaN), rounded to
+ * `dtype`.  The integer sum is exact: K 1..131071 (int32 sums of products up to 2^14).
+ *   x    int8 [M][K], pitch ldx, xs M scales;   w  int8 [N][K], pitch ldw, ws N scales
+ *        x and w 16-byte aligned, ldx and ldw multiples of 16 (K and N are free)
+ *   bias N floats or NULL
+ *   wait_cycles, timeout_probe: as in gcdr_conv_desc (gcdr_k_status reports a wait that ran out) */
+typedef struct {
+    int64_t M;
+    int N, K;
+    const int8_t *x;
+    int64_t ldx;
+    const float *xs;
+    const int8_t *w;
+    int64_t ldw;
+    const float *ws;
+    const float *bias;
+    int relu;
+    int dtype;
+    void *out;
+    int64_t ldo;
+    long long wait_cycles;
+    int timeout_probe;
+} gcdr_i8_gemm_desc;
+GCDR_API int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream);
+
+/* The norms around a block, with its gate and residual scale, in one pass:
+ *
+ *   v = x + res_scale * gate[t / gate_rows] * N1(f)       r = v
+ *   h = N2(v)                                             y = h;  q, qs = h as gcdr_k_quant_rows
+ *
+ * N1, N2 (post, pre): GCDR_NORM_LAYER (u - mean) / sqrt(var + eps) * g + b, GCDR_NORM_RMS
+ * u / sqrt(mean(u^2) + eps) * g + b, or none; g and b are C floats, NULL: 1 and 0.  Everything is held
+ * in fp32 (squares have to fit it) and rounded once, where it is stored: N2 sees v unrounded.
+ *   x     residual stream, or NULL (none added);  f  the block's output, or NULL (v = x)
+ *   gate  rows of C, row t / gate_rows for token t: gate_rows = rows one layer scale for all, tokens
+ *         per sequence a gate for each, 1 a gate for each token; NULL: 1
+ *   r, y, q + qs  each optional, at least one;  x, f, gate, r, y are of `dtype`; C 1..32768 */
+typedef struct {
+    int64_t rows;
+    int C, dtype;
+    const void *x;
+    int64_t ldx;
+    const void *f;
+    int64_t ldf;
+    int post;
+    const float *g1, *b1;
+    float eps1;
+    const void *gate;
+    int64_t ldg, gate_rows;
+    float res_scale;
+    void *r;
+    int64_t ldr;
+    int pre;
+    const float *g2, *b2;
+    float eps2;
+    void *y;
+    int64_t ldy;
+    int8_t *q;
+    int64_t ldq;
+    float *qs;
+} gcdr_block_norm_desc;
+GCDR_API int gcdr_k_block_norm(const gcdr_block_norm_desc *d, void *stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,8 @@ import io
 import os
 import threading
 
-__all__ = ["GcdrBackend", "GcdrPixelFormat", "GcdrEnhancer", "CudaWorker", "ConvDesc", "lib", "library_path",
+__all__ = ["GcdrBackend", "GcdrPixelFormat", "GcdrEnhancer", "CudaWorker", "ConvDesc", "I8GemmDesc",
+           "BlockNormDesc", "check", "lib", "library_path",
            "register_host", "unregister_host", "GcdrError", "ArgumentError", "ArgumentOutOfRangeError", "NotSupportedError",
            "DeviceLostError", "DeviceTimeoutError", "ModelError", "OutOfMemoryError",
            "bytes_per_pixel"]
@@ -106,6 +107,31 @@ class ConvDesc(ctypes.Structure):
                 ("bias_host", ctypes.c_void_p), ("wait_cycles", ctypes.c_longlong), ("timeout_probe", ctypes.c_int)]
 
 
+class I8GemmDesc(ctypes.Structure):
+    """gcdr_i8_gemm_desc of include/gcdr_cuda.h (gcdr_k_i8_gemm: int8 tokens x int8 weights, a scale each)."""
+    _fields_ = [("M", ctypes.c_int64), ("N", ctypes.c_int), ("K", ctypes.c_int), ("x", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("xs", ctypes.c_void_p), ("w", ctypes.c_void_p), ("ldw", ctypes.c_int64),
+                ("ws", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("relu", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("wait_cycles", ctypes.c_longlong),
+                ("timeout_probe", ctypes.c_int)]
+
+
+class BlockNormDesc(ctypes.Structure):
+    """gcdr_block_norm_desc of include/gcdr_cuda.h (gcdr_k_block_norm: the norms, gate and residual of a block)."""
+    _fields_ = [("rows", ctypes.c_int64), ("C", ctypes.c_int), ("dtype", ctypes.c_int), ("x", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("f", ctypes.c_void_p), ("ldf", ctypes.c_int64), ("post", ctypes.c_int),
+                ("g1", ctypes.c_void_p), ("b1", ctypes.c_void_p), ("eps1", ctypes.c_float), ("gate", ctypes.c_void_p),
+                ("ldg", ctypes.c_int64), ("gate_rows", ctypes.c_int64), ("res_scale", ctypes.c_float),
+                ("r", ctypes.c_void_p), ("ldr", ctypes.c_int64), ("pre", ctypes.c_int), ("g2", ctypes.c_void_p),
+                ("b2", ctypes.c_void_p), ("eps2", ctypes.c_float), ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
+                ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("qs", ctypes.c_void_p)]
+
+
+def check(status: int) -> None:
+    """Raises the exception of a GCDR_* status of the layer entries (nothing for GCDR_OK)."""
+    _raise(status)
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -168,6 +194,9 @@ def lib():
         L.gcdr_k_dw_gelu_shift.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp]
         L.gcdr_k_up_add.argtypes = [vp, vp, vp, vp, vp, f, vp, vp, vp]
         L.gcdr_k_ln_finalize.argtypes = [vp, i, i, i, i, vp, vp, vp, vp, f, vp, vp, f, vp, vp, vp, vp]
+        L.gcdr_k_quant_rows.argtypes = [vp, i, i64, i, i64, vp, i64, vp, vp]
+        L.gcdr_k_i8_gemm.argtypes = [vp, vp]
+        L.gcdr_k_block_norm.argtypes = [vp, vp]
         _lib = L
         return L
 

@@ -22,6 +22,7 @@
 
 #include "../../../include/gcdr_cuda.h"
 #include "conv_launch.h"
+#include "int8.h"
 #include "kernels.h"
 #include "model.h"
 #include "pipeline.h"
@@ -688,6 +689,7 @@ extern "C" int gcdr_k_status(void *stream) {
     if (cudaMemcpy(&h, d_err, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess ||
         cudaMemset(d_err, 0, sizeof(int)) != cudaSuccess)
         return GCDR_ERR_DEVICE;
+    h |= i8_status_word();
     return (h & GCDR_ERR_FLAG_TIMEOUT) ? GCDR_ERR_TIMEOUT : h ? GCDR_ERR_DEVICE : GCDR_OK;
 }
 
