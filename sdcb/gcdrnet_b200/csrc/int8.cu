@@ -84,21 +84,7 @@ int check_operands(const char *who, std::initializer_list<Operand> ops) {
 
 namespace {
 
-__device__ int g_i8_err;   // set by a kernel whose bounded wait ran out (GCDR_ERR_FLAG_*)
-
-struct I8Args {
-    int64_t M;
-    int N, K;
-    const int8_t *x;
-    int64_t ldx;
-    const float *xs;
-    const int8_t *w;
-    int64_t ldw;
-    const float *ws, *bias;
-    int relu;
-    void *out;
-    int64_t ldo;
-};
+constexpr int kDotTokens = 4;
 
 __device__ __forceinline__ float scaled(int acc, float xs, float ws, float bias, int relu) {
     const float v = fmaf((float)acc * xs, ws, bias);
@@ -161,17 +147,6 @@ cudaError_t launch_dot(const I8Args &a, cudaStream_t st) {
 
 }  // namespace
 
-int i8_status_word() {
-    int h = 0;
-    const int zero = 0;
-    if (cudaMemcpyFromSymbol(&h, g_i8_err, sizeof h) != cudaSuccess ||
-        (h && cudaMemcpyToSymbol(g_i8_err, &zero, sizeof zero) != cudaSuccess)) {
-        cudaGetLastError();
-        return GCDR_ERR_FLAG_OTHER;
-    }
-    return h;
-}
-
 }  // namespace gcdr
 
 using namespace gcdr;
@@ -195,8 +170,14 @@ extern "C" int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream) {
                                         {"bias", d->bias, 1, d->N, d->N, 4, kIn},
                                         {"out", d->out, d->M, d->N, d->ldo, size, kOut}});
     if (rc) return rc;
-    I8Args a = {d->M, d->N, d->K, d->x, d->ldx, d->xs, d->w, d->ldw, d->ws, d->bias, d->relu, d->out, d->ldo};
+    if (d->ldx >= (int64_t)1 << 40 || d->ldw >= (int64_t)1 << 40) return refuse(who, GCDR_ERR_RANGE, "a pitch of 2^40 or more");
+    const I8Args a = {d->M, d->N, d->K, d->x, d->ldx, d->xs, d->w, d->ldw, d->ws, d->bias, d->relu, d->dtype, d->out, d->ldo,
+                      d->wait_cycles, d->timeout_probe != 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.M > kDotTokens || a.timeout_probe) {
+        std::string err;
+        return i8_tc_launch(a, st, err) ? refuse(who, GCDR_ERR_DEVICE, err.c_str()) : GCDR_OK;
+    }
     const cudaError_t e = d->dtype == GCDR_DTYPE_F16    ? launch_dot<__half>(a, st)
                           : d->dtype == GCDR_DTYPE_BF16 ? launch_dot<__nv_bfloat16>(a, st)
                                                         : launch_dot<float>(a, st);

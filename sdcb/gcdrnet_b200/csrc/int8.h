@@ -1,5 +1,10 @@
-// int8.h -- what capi.cu needs of the int8 product (int8.cu).
+// int8.h -- the int8 token product (gcdr_k_i8_gemm): its arguments, its two kernels' launches, and what
+// capi.cu needs of it.
 #pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <string>
 
 namespace gcdr {
 
@@ -7,5 +12,24 @@ constexpr int GCDR_ERR_FLAG_OTHER = 1 << 30;   // the status itself could not be
 
 // Reads and clears the current device's error word of the int8 product (GCDR_ERR_FLAG_*).
 int i8_status_word();
+
+struct I8Args {
+    int64_t M;
+    int N, K;
+    const int8_t *x;
+    int64_t ldx;
+    const float *xs;
+    const int8_t *w;
+    int64_t ldw;
+    const float *ws, *bias;
+    int relu, dtype;
+    void *out;
+    int64_t ldo;
+    long long wait_cycles;
+    int timeout_probe;
+};
+
+// The tensor-core kernel (int8_tc.cu); 0, or -1 and why not.
+int i8_tc_launch(const I8Args &a, cudaStream_t st, std::string &err);
 
 }  // namespace gcdr

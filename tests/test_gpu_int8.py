@@ -527,3 +527,38 @@ def test_refusals_with_device_operands():
     assert block_norm(x=x, pre=RMS, r=both[:, :64], y=both[:, 56:120]) == 1
     assert block_norm(x=x, pre=RMS, r=both[:, :64], y=both[:, :64]) == 1
     torch.cuda.synchronize()
+
+
+# (M, N, K): a split narrow product (clusters), a narrow one, wide ones of one and of several tiles a CTA
+I8_CASES = [(20, 128, 2048), (40, 20000, 96), (200, 130, 300), (6000, 600, 256)]
+
+
+@pytest.mark.parametrize("case", I8_CASES, ids=lambda c: "%dx%dx%d" % c)
+def test_i8_gemm_wait_runs_out_and_reports_timeout(case):
+    """The test hook issues no copies and no MMAs: every role's first wait runs out, nothing is written, the
+    status says so once, and the next call is right."""
+    import time
+
+    import torch
+    from sdcb.gcdrnet_b200 import lib
+    L = lib()
+    M, N, K = case
+    g = torch.Generator(device="cuda:0").manual_seed(M)
+    x = torch.zeros(M, -(-K // 16) * 16, dtype=torch.int8, device="cuda:0")[:, :K]
+    w = torch.zeros(N, x.stride(0), dtype=torch.int8, device="cuda:0")[:, :K]
+    x.copy_(torch.randint(-127, 128, (M, K), generator=g, device="cuda:0"))
+    w.copy_(torch.randint(-127, 128, (N, K), generator=g, device="cuda:0"))
+    xs, ws = torch.ones(M, device="cuda:0"), torch.ones(N, device="cuda:0")
+    out = torch.full((M, N), float("nan"), dtype=torch.float32, device="cuda:0")
+    torch.cuda.synchronize()
+    assert L.gcdr_k_status(None) == 0
+    t0 = time.perf_counter()
+    assert i8_gemm(x, xs, w, ws, None, out, wait_cycles=400_000, timeout_probe=1) == 0
+    assert L.gcdr_k_status(None) == 5
+    assert time.perf_counter() - t0 < 5.0
+    assert torch.isnan(out).all().item(), "the probe wrote outputs"
+    assert L.gcdr_k_status(None) == 0
+    assert i8_gemm(x, xs, w, ws, None, out) == 0
+    assert L.gcdr_k_status(None) == 0
+    want, bound = ref_product(x, xs, w, ws, None, False, torch.float32)
+    assert worst(out, want, bound) <= 1.0
