@@ -24,7 +24,7 @@ FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", 
          "--expt-relaxed-constexpr", "-I", SRC, "-I", INCLUDE]
 
 SOURCES = ["model.cpp", "conv_tc.cu", "conv_rw.cu", "conv_ref.cu", "kernels.cu", "pipeline.cu", "capi.cu", "noalloc.cu",
-           "rows.cu", "int8.cu", "int8_tc.cu"]
+           "rows.cu", "rows_f16.cu", "rows_bf16.cu", "rows_f32.cu", "int8.cu", "int8_tc.cu"]
 
 
 def _headers():

@@ -1,5 +1,5 @@
-// int8.h -- the int8 token product (gcdr_k_i8_gemm): its arguments, its two kernels' launches, and what
-// capi.cu needs of it.
+// int8.h -- the int8 token product (gcdr_k_i8_gemm): its arguments, its tensor-core kernel's launch, and the
+// status word that capi.cu reads.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>

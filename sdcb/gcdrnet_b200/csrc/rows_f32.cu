@@ -1,0 +1,7 @@
+// rows_f32.cu -- the row operators on fp32 activations.
+#include "rows_kernel.cuh"
+
+namespace gcdr {
+template cudaError_t rows_launch<float, true>(const RowArgs &, bool, cudaStream_t);
+template cudaError_t rows_launch<float, false>(const RowArgs &, bool, cudaStream_t);
+}  // namespace gcdr
