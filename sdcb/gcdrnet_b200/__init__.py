@@ -139,6 +139,8 @@ _lib_lock = threading.Lock()
 def lib():
     """The loaded libgcdr_cuda.so (raises when it has not been built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lib_lock:
         if _lib is not None:
             return _lib

@@ -100,49 +100,80 @@ __device__ __forceinline__ int4 load16(const int8_t *row, int k, int K) {
     return make_int4(w[0], w[1], w[2], w[3]);
 }
 
-// A warp forms the products of one channel with MT tokens: the lanes take the row 16 bytes each.
-template <class T, int MT>
-__global__ void __launch_bounds__(256) i8_dot_kernel(const __grid_constant__ I8Args a) {
+// A warp forms the products of R channels with MT tokens, the lanes 16 bytes of a row each: U pieces of every row
+// are on their way at once, each token's piece serves R channels.
+template <class T, int MT, int R, int U>
+__global__ void __launch_bounds__(128) i8_dot_kernel(const __grid_constant__ I8Args a) {
     const int lane = threadIdx.x & 31;
-    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t n0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * R;
     pdl_wait();
-    if (n < a.N) {
-        const int8_t *w = a.w + n * a.ldw;
-        const float ws = a.ws[n], bias = a.bias ? a.bias[n] : 0.f;
-        for (int64_t m0 = (int64_t)blockIdx.y * MT; m0 < a.M; m0 += (int64_t)gridDim.y * MT) {
-            int acc[MT];
+    if (n0 < a.N) {
+        int acc[R][MT];
+        const int8_t *w[R], *x[MT];
 #pragma unroll
-            for (int j = 0; j < MT; j++) acc[j] = 0;
-            for (int k = lane * 16; k < a.K; k += 512) {
-                const int4 b = load16(w, k, a.K);
+        for (int r = 0; r < R; r++) w[r] = a.w + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ldw;   // (a row twice, not past the last)
 #pragma unroll
-                for (int j = 0; j < MT; j++) {
-                    if (m0 + j >= a.M) break;
-                    const int4 x = load16(a.x + (m0 + j) * a.ldx, k, a.K);
-                    acc[j] = __dp4a(x.x, b.x, acc[j]);
-                    acc[j] = __dp4a(x.y, b.y, acc[j]);
-                    acc[j] = __dp4a(x.z, b.z, acc[j]);
-                    acc[j] = __dp4a(x.w, b.w, acc[j]);
-                }
-            }
+        for (int j = 0; j < MT; j++) x[j] = a.x + (j < a.M ? j : a.M - 1) * a.ldx;
 #pragma unroll
-            for (int j = 0; j < MT; j++) {
-                if (m0 + j >= a.M) break;
-                const int sum = __reduce_add_sync(0xFFFFFFFFu, acc[j]);
-                if (lane == 0)
-                    static_cast<T *>(a.out)[(m0 + j) * a.ldo + n] = from_f32<T>(scaled(sum, a.xs[m0 + j], ws, bias, a.relu));
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) acc[r][j] = 0;
+        const auto dot = [&](const int4 &p, const int4 &q, int &sum) {
+            sum = __dp4a(p.x, q.x, sum);
+            sum = __dp4a(p.y, q.y, sum);
+            sum = __dp4a(p.z, q.z, sum);
+            sum = __dp4a(p.w, q.w, sum);
+        };
+        int k = lane * 16;
+        for (; k - lane * 16 + U * 512 <= a.K; k += U * 512) {
+            int4 p[R][U], q[MT];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int r = 0; r < R; r++) p[r][u] = __ldcs(reinterpret_cast<const int4 *>(w[r] + k + u * 512));
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+#pragma unroll
+                for (int j = 0; j < MT; j++) q[j] = *reinterpret_cast<const int4 *>(x[j] + k + u * 512);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int j = 0; j < MT; j++) dot(p[r][u], q[j], acc[r][j]);
             }
         }
+        for (; k < a.K; k += 512) {
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const int4 p = load16(w[r], k, a.K);
+#pragma unroll
+                for (int j = 0; j < MT; j++) dot(p, load16(x[j], k, a.K), acc[r][j]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                const int sum = __reduce_add_sync(0xFFFFFFFFu, acc[r][j]);
+                if (lane == 0 && j < a.M && n0 + r < a.N)
+                    static_cast<T *>(a.out)[j * a.ldo + n0 + r] =
+                        from_f32<T>(scaled(sum, a.xs[j], a.ws[n0 + r], a.bias ? a.bias[n0 + r] : 0.f, a.relu));
+            }
     }
     pdl_trigger();
 }
 
+template <class T, int MT, int R, int U>
+cudaError_t launch_dot(const I8Args &a, cudaStream_t st) {
+    return launch_pdl(i8_dot_kernel<T, MT, R, U>, dim3((unsigned)(((int64_t)a.N + 4 * R - 1) / (4 * R))), dim3(128), 0, st, a);
+}
+
 template <class T>
 cudaError_t launch_dot(const I8Args &a, cudaStream_t st) {
-    constexpr int MT = 4;
-    const int64_t my = (a.M + MT - 1) / MT;
-    const dim3 grid((unsigned)(((int64_t)a.N + 7) / 8), (unsigned)(my < 65535 ? my : 65535));
-    return launch_pdl(i8_dot_kernel<T, MT>, grid, dim3(256), 0, st, a);
+    // few channels: a warp each, so that they spread over the GPU
+    const bool few = a.N < 4096;
+    if (a.M == 1) return few ? launch_dot<T, 1, 1, 4>(a, st) : launch_dot<T, 1, 2, 4>(a, st);
+    if (a.M == 2) return few ? launch_dot<T, 2, 1, 4>(a, st) : launch_dot<T, 2, 2, 4>(a, st);
+    return few ? launch_dot<T, 4, 1, 4>(a, st) : launch_dot<T, 4, 2, 4>(a, st);
 }
 
 }  // namespace

@@ -1,20 +1,22 @@
 // int8_tc.cu -- the int8 token product on the 5th-generation tensor cores (sm_100a).
 //
 // tcgen05.mma.kind::i8 multiplies int8 tiles into int32 accumulators in TMEM: exact sums, whatever
-// the order.  A unit of work is a tile of 128 rows of one operand ("P", the MMA's M) times bn rows of
+// the order.  A unit of work is a tile of 128 or 256 rows of one operand ("P", the MMA's M) times bn rows of
 // the other ("Q", its N), K in blocks of 128 bytes:
 //
 //   wide form     P = tokens, Q = channels.  A thread of the epilogue holds a token's results in a row;
 //                 they go through a per-warp stage in shared memory, so that a store instruction writes
-//                 64 neighbouring bytes of eight tokens instead of 16 bytes of 32.
+//                 whole lines or halves.  Units of 256 rows are shared by the two CTAs of a cluster
+//                 (cta_group::2): each loads 128 rows of P and half of Q, one issues the MMAs for both.
 //   narrow form   P = channels, Q = tokens (few of them): the weights' rows fill the 128 MMA rows that
 //                 few tokens would leave empty, and a warp's 32 channels are neighbours in the result.
 //                 K is split over the CTAs of a cluster when the tiles do not fill the GPU: their int32
 //                 sums are joined through distributed shared memory, each CTA finishing a share of the
 //                 tokens.  (Integers: the join is exact and the same at any split.)
 //
-// 12 warps: TMA producer, MMA issuer, TMEM allocation, one idle, 8 epilogue warps (two per TMEM lane
-// quadrant).  Accumulators are double-buffered in TMEM: a unit's epilogue runs under the next one's MMAs.
+// 4 + EPI warps: TMA producer, MMA issuer, TMEM allocation, one idle, and the epilogue warps, which read the TMEM lane
+// quadrant of their number.  TMEM holds up to four accumulators; in the wide form each has its own group of epilogue
+// warps, so that several units' epilogues, whose latencies add up to more than a unit's MMAs, run side by side.
 // The tail of K and rows past an operand's end arrive as zeros (TMA fill).  Every mbarrier wait is
 // bounded, as in conv_tc.cu.
 #include <cuda.h>
@@ -34,19 +36,24 @@ namespace {
 
 __device__ int g_i8_err;   // set by a kernel whose bounded wait ran out (GCDR_ERR_FLAG_*)
 
-constexpr int kEpiWarps = 8;
 constexpr int kFirstEpi = 4;
-constexpr int kThreads = (kFirstEpi + kEpiWarps) * 32;
 constexpr int kBlockK = 128;                       // bytes of K per ring stage (one 128-byte swizzle row)
 constexpr int kRingStages = 12;
+constexpr int kMaxBufs = 4;                        // accumulators in TMEM
 constexpr int kPBytes = 128 * kBlockK;
-constexpr int kStageBytes = 2048;                  // an epilogue warp's store stage: 32 rows of 64 bytes
+// An epilogue warp's store stage: 32 rows of a 128-byte line where the stores bound the launch (16 warps), of half of
+// it where a unit's latency counts (8 warps: more of them share a unit's columns).
+__host__ __device__ constexpr int row_bytes(int epi) { return epi == 16 ? 128 : 64; }
+constexpr int kScaleBytes = 8192;                  // channel scales and biases: two sets per accumulator
 constexpr int kSmemCap = 227 * 1024;
 constexpr int kXchPitch = 129;                     // int32 words per column of the split's exchange (odd: no bank conflicts)
 
 struct I8Plan {
     int narrow;          // P = channels
+    int pair;            // units of 256 rows, two CTAs each (wide form)
+    int epi;             // epilogue warps: 8 or 16
     int bn;              // rows of Q per unit
+    int bufs;            // accumulators
     int split;           // CTAs per cluster, each a share of K (narrow form)
     int stages;
     int kblocks;
@@ -56,7 +63,7 @@ struct I8Plan {
 };
 
 struct I8Shared {
-    uint64_t full[kRingStages], empty[kRingStages], tfull[2], tempty[2], mdone;
+    uint64_t full[kRingStages], empty[kRingStages], tfull[kMaxBufs], tempty[kMaxBufs], mdone;
     uint32_t tmem_base;
     int abort_flag, peer_abort;
     int issued, consumed;
@@ -79,22 +86,83 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, int v) {
     asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *m) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+
 // D = int32, A and B signed int8, both K-major, N >> 3 at [17, 23), M >> 4 at [24, 29)
 __device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+template <int CG>
 __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accum));
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accum));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accum));
 }
 
-__device__ __forceinline__ float scaled(int acc, float xs, float ws, float bias, int relu) {
+// The MMAs issued so far arrive on `bar` when they are done: in the pair form on that barrier of both CTAs.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        mma_commit(bar);
+}
+
+// A box of one of the pair's CTAs, counted by the leader's barrier (`bar`: its shared::cluster address)
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+template <int CG>
+__device__ __forceinline__ void alloc_tmem(uint32_t *slot, uint32_t cols) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tmem_alloc(slot, cols);
+    }
+}
+template <int CG>
+__device__ __forceinline__ void free_tmem(uint32_t base, uint32_t cols) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+    else
+        tmem_dealloc(base, cols);
+}
+
+__device__ __forceinline__ float scaled(int acc, float xs, float ws, float bias, bool relu) {
     const float v = fmaf((float)acc * xs, ws, bias);
     return relu && v < 0.f ? 0.f : v;   // (a NaN stays)
+}
+
+// max(v, 0), a NaN stays
+__device__ __forceinline__ float relu(float v) {
+    float m;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(m) : "f"(v));
+    return m;
 }
 
 // Unit u -> its P and Q tiles: `group` P tiles per Q tile, then the next Q tile.
@@ -107,33 +175,42 @@ __device__ __forceinline__ void unit_tiles(const I8Plan &pl, int u, int &pt, int
     pt = g * pl.group + r - qt * n;
 }
 
-template <class T, bool NARROW>
-__global__ void __launch_bounds__(kThreads, 1)
+// CG: CTAs per unit.  EPI: epilogue warps.
+template <class T, bool NARROW, int CG, int EPI>
+__global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
     i8_tc_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
                  const __grid_constant__ I8Args a, const __grid_constant__ I8Plan pl) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int bn = pl.bn;
-    const int stage_bytes = kPBytes + bn * kBlockK;
+    const int stage_bytes = kPBytes + bn / CG * kBlockK;
     uint8_t *extra = ring + (size_t)pl.stages * stage_bytes;
     I8Shared *sh = reinterpret_cast<I8Shared *>(extra + pl.extra_bytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = NARROW ? pl.split : 1;
-    const uint32_t rank = split > 1 ? cluster_rank() : 0;
-    const int first = blockIdx.x / split, stride = gridDim.x / split;
+    const int cluster = CG == 2 ? 2 : split;
+    const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
+    const int first = blockIdx.x / cluster, stride = gridDim.x / cluster;
     const int units = pl.tiles_p * pl.tiles_q;
-    const int kb0 = (int)((long long)pl.kblocks * rank / split), kb1 = (int)((long long)pl.kblocks * (rank + 1) / split);
-    const uint32_t tmem_cols = 2u * bn;
+    const int kb0 = NARROW ? (int)((long long)pl.kblocks * rank / split) : 0;
+    const int kb1 = NARROW ? (int)((long long)pl.kblocks * (rank + 1) / split) : pl.kblocks;
+    const uint32_t tmem_cols = (uint32_t)(pl.bufs * bn);
+    // epilogue warps of an accumulator: all of them in the narrow form, else a group of its own
+    const int per_buf = NARROW ? EPI : EPI / pl.bufs;
 
+    if (threadIdx.x == 32) {             // the tensor maps are on their way while the previous kernel ends
+        prefetch_map(&tmP);
+        prefetch_map(&tmQ);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < pl.stages; s++) {
             mbar_init(&sh->full[s], 1);
             mbar_init(&sh->empty[s], 1);
         }
-        for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < pl.bufs; b++) {
             mbar_init(&sh->tfull[b], 1);
-            mbar_init(&sh->tempty[b], kEpiWarps);
+            mbar_init(&sh->tempty[b], (uint32_t)(per_buf * CG));
         }
         mbar_init(&sh->mdone, 1);
         sh->abort_flag = sh->peer_abort = 0;
@@ -142,11 +219,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == 2) {
         __syncwarp();
-        tmem_alloc(&sh->tmem_base, tmem_cols);
+        alloc_tmem<CG>(&sh->tmem_base, tmem_cols);
     }
     tc_fence_before();
     __syncthreads();
-    if (split > 1) cluster_sync();       // the other CTAs run: their shared memory may be written
+    if (cluster > 1) cluster_sync();     // the other CTAs run and have their barriers: they may be written to
     tc_fence_after();
     const uint32_t tmem_base = sh->tmem_base;
     volatile int *abort_flag = &sh->abort_flag;
@@ -165,9 +242,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int kb = kb0; kb < kb1; kb++) {
                     if (!mbar_wait(&sh->empty[s], ph ^ 1u, abort_flag, &g_i8_err, budget)) { ok = false; break; }
                     uint8_t *st = ring + (size_t)s * stage_bytes;
-                    mbar_expect_tx(&sh->full[s], (uint32_t)stage_bytes);
-                    tma_load_2d(st, &tmP, kb * kBlockK, pt * 128, &sh->full[s]);
-                    tma_load_2d(st + kPBytes, &tmQ, kb * kBlockK, qt * bn, &sh->full[s]);
+                    if constexpr (CG == 2) {
+                        const uint32_t bar = map_to(smem_u32(&sh->full[s]), 0);
+                        if (rank == 0) mbar_expect_tx(&sh->full[s], 2u * (uint32_t)stage_bytes);
+                        tma_load_pair(st, &tmP, kb * kBlockK, pt * 256 + (int)rank * 128, bar);
+                        tma_load_pair(st + kPBytes, &tmQ, kb * kBlockK, qt * bn + (int)rank * (bn / 2), bar);
+                    } else {
+                        mbar_expect_tx(&sh->full[s], (uint32_t)stage_bytes);
+                        tma_load_2d(st, &tmP, kb * kBlockK, pt * 128, &sh->full[s]);
+                        tma_load_2d(st + kPBytes, &tmQ, kb * kBlockK, qt * bn, &sh->full[s]);
+                    }
                     issued++;
                     if (++s == pl.stages) { s = 0; ph ^= 1u; }
                 }
@@ -175,15 +259,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             sh->issued = issued;
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && (CG == 1 || rank == 0)) {
             const uint64_t desc0 = sdesc(0, 8 * kBlockK, 2);
-            const uint32_t idesc = idesc_i8(128, bn);
-            int s = 0, t = 0, consumed = 0;
-            uint32_t ph = 0;
+            const uint32_t idesc = idesc_i8(128 * CG, bn);
+            int s = 0, ab = 0, consumed = 0;
+            uint32_t ph = 0, aph = 0;
             bool ok = true;
-            for (int u = first; u < units && ok; u += stride, t++) {
-                const int ab = t & 1;
-                if (!mbar_wait(&sh->tempty[ab], (uint32_t)((t >> 1) & 1) ^ 1u, abort_flag, &g_i8_err, budget)) break;
+            for (int u = first; u < units && ok; u += stride) {
+                if (!mbar_wait(&sh->tempty[ab], aph ^ 1u, abort_flag, &g_i8_err, budget)) break;
+                if (CG == 2) fence_acquire_cluster();    // the other CTA's epilogue has read its half
                 tc_fence_after();
                 const uint32_t d = tmem_base + (uint32_t)(ab * bn);
                 for (int kb = kb0; kb < kb1; kb++) {
@@ -194,58 +278,82 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint64_t bd = desc0 | (uint64_t)(((st + kPBytes) & 0x3FFFFu) >> 4);
 #pragma unroll
                     for (int k = 0; k < kBlockK / 32; k++)
-                        mma_i8(d, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc, (kb > kb0 || k) ? 1u : 0u);
-                    mma_commit(&sh->empty[s]);
+                        mma_i8<CG>(d, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc, (kb > kb0 || k) ? 1u : 0u);
+                    commit<CG>(&sh->empty[s]);
                     consumed++;
                     if (++s == pl.stages) { s = 0; ph ^= 1u; }
                 }
-                if (ok) mma_commit(&sh->tfull[ab]);
+                if (ok) commit<CG>(&sh->tfull[ab]);
+                if (++ab == pl.bufs) { ab = 0; aph ^= 1u; }
             }
             sh->consumed = consumed;
             if (*abort_flag) {   // every MMA issued is done (bounded) before TMEM is freed
-                mma_commit(&sh->mdone);
+                commit<CG>(&sh->mdone);
                 const long long t0 = clock64();
                 while (!mbar_try(&sh->mdone, 0) && clock64() - t0 < kWaitCycles) {}
             }
         }
     } else if (warp >= kFirstEpi) {
-        const int e = warp - kFirstEpi, quad = warp & 3, part = e >> 2;
+        const int e = warp - kFirstEpi, quad = warp & 3;
+        const int group = NARROW ? 0 : e / per_buf, parts = per_buf / 4, part = (e - group * per_buf) >> 2;
+        const int gi = (int)threadIdx.x - (kFirstEpi + group * per_buf) * 32;   // thread of the group
         const int row = quad * 32 + lane;
         const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
-        int t = 0;
-        for (int u = first; u < units; u += stride, t++) {
+        float *scales = reinterpret_cast<float *>(extra + EPI * 32 * row_bytes(EPI)) + group * 4 * bn;
+        // a unit's scales: of this thread's row, and (wide) of one or two channels for the group; those of the group's
+        // next unit are fetched while this one is finished
+        constexpr int CH = NARROW || EPI == 16 ? 1 : 2;
+        float rs = 0.f, rb = 0.f, cs[CH], cb[CH];
+        const auto fetch_scales = [&](int u) {
             int pt, qt;
             unit_tiles(pl, u, pt, qt);
-            const int ab = t & 1;
-            const int64_t n0 = NARROW ? (int64_t)pt * 128 : (int64_t)qt * bn;
-            const int64_t m0 = NARROW ? (int64_t)qt * bn : (int64_t)pt * 128;
-            // the tile's channel scales and biases, before its sums arrive
-            float *sc = reinterpret_cast<float *>(extra + kEpiWarps * kStageBytes) + ab * 512;
-            float rs = 0.f, rb = 0.f;
             if (NARROW) {
-                if (n0 + row < a.N) {
-                    rs = a.ws[n0 + row];
-                    rb = a.bias ? a.bias[n0 + row] : 0.f;
-                }
+                const int64_t n = (int64_t)pt * 128 + row;
+                rs = n < a.N ? a.ws[n] : 0.f;
+                rb = n < a.N && a.bias ? a.bias[n] : 0.f;
             } else {
-                const int i = threadIdx.x - kFirstEpi * 32;
-                if (i < bn) {
-                    const bool in = n0 + i < a.N;
-                    sc[i] = in ? a.ws[n0 + i] : 0.f;
-                    sc[256 + i] = in && a.bias ? a.bias[n0 + i] : 0.f;
+                const int64_t m = ((int64_t)pt * CG + rank) * 128 + row;
+                rs = m < a.M ? a.xs[m] : 0.f;
+#pragma unroll
+                for (int i = 0; i < CH; i++) {
+                    const int c = gi + i * per_buf * 32;
+                    const int64_t n = (int64_t)qt * bn + c;
+                    cs[i] = c < bn && n < a.N ? a.ws[n] : 0.f;
+                    cb[i] = c < bn && n < a.N && a.bias ? a.bias[n] : 0.f;
                 }
-                if (m0 + row < a.M) rs = a.xs[m0 + row];
             }
-            const bool ok = mbar_wait(&sh->tfull[ab], (uint32_t)((t >> 1) & 1), abort_flag, &g_i8_err, budget);
-            // the epilogue warps go on or leave together
+        };
+        const int step = NARROW ? 1 : pl.bufs;
+        int ab = group, odd = 0;
+        uint32_t aph = 0;
+        if (first + group * stride < units) fetch_scales(first + group * stride);
+        for (int u = first + group * stride; u < units; u += step * stride) {
+            int pt, qt;
+            unit_tiles(pl, u, pt, qt);
+            const int64_t n0 = NARROW ? (int64_t)pt * 128 : (int64_t)qt * bn;
+            const int64_t m0 = NARROW ? (int64_t)qt * bn : ((int64_t)pt * CG + rank) * 128;
+            float *sc = scales + odd * 2 * bn;     // (the other set may still be read)
+            odd ^= 1;
+            const float row_s = rs, row_b = rb;
+#pragma unroll
+            for (int i = 0; !NARROW && i < CH; i++) {
+                const int c = gi + i * per_buf * 32;
+                if (c < bn) {
+                    sc[c] = cs[i];
+                    sc[bn + c] = cb[i];
+                }
+            }
+            if (u + step * stride < units) fetch_scales(u + step * stride);
+            const bool ok = mbar_wait(&sh->tfull[ab], aph, abort_flag, &g_i8_err, budget);
+            // the accumulator's warps go on or leave together
             uint32_t bad;
             asm volatile(
                 "{\n\t.reg .pred p, q;\n\t"
                 "setp.eq.u32 p, %1, 0;\n\t"
-                "bar.red.or.pred q, 1, %2, p;\n\t"
+                "bar.red.or.pred q, %2, %3, p;\n\t"
                 "selp.u32 %0, 1, 0, q;\n\t}"
                 : "=r"(bad)
-                : "r"((uint32_t)ok), "n"(kEpiWarps * 32)
+                : "r"((uint32_t)ok), "r"(1 + group), "r"(per_buf * 32)
                 : "memory");
             if (bad) break;
             tc_fence_after();
@@ -254,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // to the CTA that finishes these tokens: its slot of this CTA, [token][channel]
                 const uint32_t own = smem_u32(extra);
                 const int cols = (bn + split - 1) / split;
-                for (int c0 = part * 16; c0 < bn && m0 + c0 < a.M; c0 += 32) {
+                for (int c0 = part * 16; c0 < bn && m0 + c0 < a.M; c0 += parts * 16) {
                     uint32_t r[16];
                     ld.load16_nw(r, c0);
                     TmemLoader::wait_ld();
@@ -268,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else if (NARROW) {
                 T *out = static_cast<T *>(a.out);
-                for (int c0 = part * 16; c0 < bn && m0 + c0 < a.M; c0 += 32) {
+                for (int c0 = part * 16; c0 < bn && m0 + c0 < a.M; c0 += parts * 16) {
                     uint32_t r[16];
                     ld.load16_nw(r, c0);
                     TmemLoader::wait_ld();
@@ -276,66 +384,93 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int j = 0; j < 16; j++) {
                         const int64_t m = m0 + c0 + j;
                         if (m >= a.M) break;
-                        const float v = scaled((int)r[j], a.xs[m], rs, rb, a.relu);
+                        const float v = scaled((int)r[j], a.xs[m], row_s, row_b, a.relu);
                         if (n0 + row < a.N) out[m * a.ldo + n0 + row] = from_f32<T>(v);
                     }
                 }
             } else {
-                constexpr int CW = 64 / (int)sizeof(T);       // columns of a store stage
-                constexpr int E = 16 / (int)sizeof(T);        // elements of a 16-byte store
-                uint8_t *stg = extra + e * kStageBytes;
+                constexpr int E = 16 / (int)sizeof(T);        // elements of a 16-byte piece
+                constexpr int RB = row_bytes(EPI), PC = RB / 16;   // bytes and pieces of a stage's row
+                constexpr int CW = PC * E, LW = CW < 32 ? CW : 32;  // its columns, those of one TMEM load
+                // pieces are stored crosswise: neither the writes (a row a lane) nor the reads (a row per PC
+                // lanes) meet in a bank
+                const auto piece = [](int r, int k) { return r * RB + ((k ^ (PC == 8 ? r & 7 : (r >> 1) & 3)) * 16); };
+                uint8_t *stg = extra + e * 32 * RB;
                 T *out = static_cast<T *>(a.out);
                 const bool vec = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.ldo * (int64_t)sizeof(T))) & 15) == 0;
                 const int64_t mb = m0 + quad * 32;
-                for (int c0 = part * CW; c0 < bn && n0 + c0 < a.N; c0 += 2 * CW) {
-                    uint32_t r[CW];
-                    ld.taddr = lane_base + (uint32_t)(ab * bn + c0);
-                    if constexpr (CW == 32) ld.load32_nw(r);
-                    else ld.load16_nw(r);
-                    TmemLoader::wait_ld();
-                    const float *ws = sc + c0, *bs = ws + 256;
+                const float2 rs2 = make_float2(row_s, row_s);
+                const int c_end = a.N - n0 < bn ? (int)(a.N - n0) : bn;
+                for (int c0 = part * CW; c0 < c_end; c0 += parts * CW) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float v[E];
+                    for (int h = 0; h < CW / LW; h++) {
+                        uint32_t r[LW];
+                        ld.taddr = lane_base + (uint32_t)(ab * bn + c0 + LW * h);
+                        if constexpr (LW == 32) ld.load32_nw(r);
+                        else ld.load16_nw(r);
+                        TmemLoader::wait_ld();
+                        const float4 *ws = reinterpret_cast<const float4 *>(sc + c0 + LW * h), *bs = ws + bn / 4;
 #pragma unroll
-                        for (int i = 0; i < E; i++) v[i] = scaled((int)r[k * E + i], rs, ws[k * E + i], bs[k * E + i], a.relu);
-                        // 16-byte pieces are stored crosswise: neither the writes (a row a lane) nor the
-                        // reads (a row per four lanes) meet in a bank
-                        uint4 *to = reinterpret_cast<uint4 *>(stg + lane * 64 + ((k ^ ((lane >> 1) & 3)) * 16));
-                        if constexpr (sizeof(T) == 4)
-                            *to = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-                        else
-                            *to = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+                        for (int k = 0; k < LW / E; k++) {
+                            uint32_t p[4];
+#pragma unroll
+                            for (int i = 0; i < E / 4; i++) {
+                                const float4 w = ws[k * (E / 4) + i], c = bs[k * (E / 4) + i];
+                                const int *q = reinterpret_cast<const int *>(r) + k * E + 4 * i;
+                                float2 v0 = __ffma2_rn(__fmul2_rn(make_float2((float)q[0], (float)q[1]), rs2), make_float2(w.x, w.y), make_float2(c.x, c.y));
+                                float2 v1 = __ffma2_rn(__fmul2_rn(make_float2((float)q[2], (float)q[3]), rs2), make_float2(w.z, w.w), make_float2(c.z, c.w));
+                                if (a.relu) {
+                                    v0 = make_float2(relu(v0.x), relu(v0.y));
+                                    v1 = make_float2(relu(v1.x), relu(v1.y));
+                                }
+                                if constexpr (sizeof(T) == 4) {
+                                    p[0] = __float_as_uint(v0.x); p[1] = __float_as_uint(v0.y);
+                                    p[2] = __float_as_uint(v1.x); p[3] = __float_as_uint(v1.y);
+                                } else {
+                                    p[2 * i] = pack2(v0.x, v0.y, T());
+                                    p[2 * i + 1] = pack2(v1.x, v1.y, T());
+                                }
+                            }
+                            *reinterpret_cast<uint4 *>(stg + piece(lane, h * (LW / E) + k)) = make_uint4(p[0], p[1], p[2], p[3]);
+                        }
                     }
                     __syncwarp();
                     const int64_t nb = n0 + c0;
                     if (vec) {
-                        const int64_t n = nb + (lane & 3) * E;
+                        const int64_t n = nb + lane % PC * E;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int r8 = i * 8 + (lane >> 2);
-                            const uint8_t *from = stg + r8 * 64 + (((lane & 3) ^ ((r8 >> 1) & 3)) * 16);
-                            if (mb + r8 < a.M) {
-                                T *to = out + (mb + r8) * a.ldo + n;
+                        for (int i = 0; i < PC; i++) {
+                            const int r = i * (32 / PC) + lane / PC;
+                            const uint8_t *from = stg + piece(r, lane % PC);
+                            if (mb + r < a.M) {
+                                T *to = out + (mb + r) * a.ldo + n;
                                 if (n + E <= a.N) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
                                 else
                                     for (int k = 0; k < E && n + k < a.N; k++) to[k] = reinterpret_cast<const T *>(from)[k];
                             }
                         }
                     } else {
-                        constexpr int RI = 32 / CW;           // rows per instruction
-                        const int c = lane % CW;
-                        for (int r0 = lane / CW; r0 < 32; r0 += RI)
-                            if (mb + r0 < a.M && nb + c < a.N)
-                                out[(mb + r0) * a.ldo + nb + c] = *reinterpret_cast<const T *>(
-                                    stg + r0 * 64 + (((c / E) ^ ((r0 >> 1) & 3)) * 16) + (c % E) * sizeof(T));
+                        // results at odd places: an element a lane, whole rows or two of them at a time
+                        constexpr int CL = CW < 32 ? CW : 32, RI = 32 / CL;
+                        for (int r = lane / CL; r < 32 && mb + r < a.M; r += RI)
+                            for (int c = lane % CL; c < CW; c += CL)
+                                if (nb + c < a.N)
+                                    out[(mb + r) * a.ldo + nb + c] =
+                                        *reinterpret_cast<const T *>(stg + piece(r, c / E) + (c % E) * sizeof(T));
                     }
                     __syncwarp();
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->tempty[ab]);
+            if (lane == 0) {
+                if (CG == 2) arrive_cluster(map_to(smem_u32(&sh->tempty[ab]), 0));
+                else mbar_arrive(&sh->tempty[ab]);
+            }
+            if (!NARROW || ++ab == pl.bufs) {
+                if (NARROW) ab = 0;
+                aph ^= 1u;
+            }
         }
     }
 
@@ -353,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t n = (int64_t)pt * 128 + row, m0 = (int64_t)qt * bn;
             if (n < a.N) {
                 const float ws = a.ws[n], bs = a.bias ? a.bias[n] : 0.f;
-                for (int at = threadIdx.x >> 7; at < cols; at += kThreads / 128) {
+                for (int at = threadIdx.x >> 7; at < cols; at += (kFirstEpi + EPI) / 4) {
                     const int64_t m = m0 + at * split + rank;
                     if (at * split + (int)rank >= bn || m >= a.M) break;
                     int sum = 0;
@@ -364,69 +499,99 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     if (threadIdx.x == 0) {
-        // copies issued but never consumed (only after an abort), then the arrivals of the last commits
-        for (int g = sh->consumed; g < sh->issued; g++) {
+        // copies issued but never consumed (only after an abort; the leader's barrier counts those of both CTAs of a
+        // pair), then the arrivals of the last commits
+        for (int g = sh->consumed; (CG == 1 || rank == 0) && g < sh->issued; g++) {
             const long long t0 = clock64();
             while (!mbar_try(&sh->full[g % pl.stages], (uint32_t)((g / pl.stages) & 1)) && clock64() - t0 < kWaitCycles) {}
         }
-        if (sh->consumed > 0) {
-            const int g = sh->consumed - 1;
+        const int done = CG == 2 && rank ? sh->issued : sh->consumed;
+        if (done > 0) {
             const long long t0 = clock64();
-            while (!mbar_try(&sh->empty[g % pl.stages], (uint32_t)((g / pl.stages) & 1)) && clock64() - t0 < kWaitCycles) {}
+            while (!mbar_try(&sh->empty[(done - 1) % pl.stages], (uint32_t)(((done - 1) / pl.stages) & 1)) && clock64() - t0 < kWaitCycles) {}
         }
     }
     __syncthreads();
+    if (CG == 2) cluster_sync();         // neither CTA's memory goes while the other's MMAs or arrivals may use it
     if (warp == 2) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem_base, tmem_cols);
+        free_tmem<CG>(tmem_base, tmem_cols);
     }
 }
 
-int pow2_at_least(int64_t v) {
-    int p = 1;
-    while (p < v) p <<= 1;
-    return p;
-}
-
+// Picks form and tile by an estimate in SM cycles, fitted to measured sweeps (B200, K 256 to 8192, 16 to 57600
+// tokens, 160 to 8192 channels; within 15 % of the best form there):
+//   a k-block step     its bytes at 50 per cycle (what an SM draws from L2), 600 at least; 680 for a pair
+//   a unit's results   at 8 bytes per cycle with 8 epilogue warps (64-byte stores), 13 with 16 of them or when the 8 share
+//                      a single unit; 16 warps start 1500 cycles later
+//   a round            400 between units; the last one's results and the start are not hidden
+//   a split of K       the join's words through distributed shared memory; clusters of eight fit the GPU 12 times
+// E.g. 57600 x 256 x 256 fp16: wide 128, 16 warps 15.6 us, 8 warps 17.5, wide 256 16.6, pair 18.5; 1800 x 512 x 512: wide
+// 64 4.6 us, 128 5.2, 16 warps 6.2; 4096^3: pair 52 us, wide 256 63, wide 128 79; 128 x 1024 x 8192: narrow 32 split 4
+// 10.9 us, wide 64 22; 16 x 2048 x 2048: split 4 6.4 us, 2 7.6, none 7.9.
 I8Plan plan_for(const I8Args &a, int sms) {
+    const auto div = [](int64_t v, int64_t d) { return (v + d - 1) / d; };
+    const int64_t kb = div(a.K, kBlockK);
+    const int size = dtype_bytes(a.dtype);
     I8Plan pl = {};
-    pl.kblocks = (a.K + kBlockK - 1) / kBlockK;
-    pl.split = 1;
-    const auto div = [](int64_t v, int d) { return (int)((v + d - 1) / d); };
-    if (a.M <= 64) {
-        pl.narrow = 1;
-        pl.bn = a.M <= 16 ? 16 : pow2_at_least(a.M);
-        pl.tiles_p = div(a.N, 128);
-        pl.tiles_q = div(a.M, pl.bn);
-        while (pl.split < 8 && 2 * pl.split <= pl.kblocks && (int64_t)pl.tiles_p * pl.tiles_q * pl.split * 2 <= sms) pl.split *= 2;
-    } else {
-        // the widest tile that still gives every SM one; 64 columns at least
-        pl.bn = 256;
-        while (pl.bn > 64 && ((int64_t)div(a.M, 128) * div(a.N, pl.bn) < sms || a.N <= pl.bn / 2)) pl.bn /= 2;
-        pl.tiles_p = div(a.M, 128);
-        pl.tiles_q = div(a.N, pl.bn);
+    int64_t best = INT64_MAX;
+    const auto offer = [&](int64_t cost, int narrow, int pair, int epi, int bn, int split) {
+        if (cost >= best) return;
+        best = cost;
+        pl.narrow = narrow;
+        pl.pair = pair;
+        pl.epi = epi;
+        pl.bn = bn;
+        pl.split = split;
+    };
+    const int64_t m128 = div(a.M, 128);
+    for (int bn = 64; bn <= 256; bn *= 2) {
+        const int64_t tq = div(a.N, bn), units = m128 * tq, rounds = div(units, sms);
+        const int64_t work = kb * (bn == 256 ? 983 : bn == 128 ? 655 : 600), bytes = 128ll * bn * size;
+        const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 400) + (w > e ? e : w); };
+        offer(cost(rounds, work, rounds == 1 ? bytes / 13 : bytes / 8) + 1500, 0, 0, 8, bn, 1);
+        if (rounds > 2) offer(cost(rounds, work, bytes / 13) + 3000, 0, 0, 16, bn, 1);
+        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * 680, bytes / 8) + 5500, 0, 1, 8, bn, 1);
+        if (a.N <= bn) break;
     }
+    const int64_t n128 = div(a.N, 128);
+    for (int bn = 16; a.M <= 512 && bn <= 128; bn *= 2) {
+        const int64_t tiles = n128 * div(a.M, bn), step = bn == 128 ? 655 : 600;
+        for (int split = 1; split <= 8 && split <= kb; split *= 2) {
+            const int64_t rounds = div(tiles * split, split == 8 ? 96 : sms);
+            offer(rounds * (div(kb, split) * step + (split > 1 ? 1500 + bn * 100 : 0)) + 4000 + bn * 30, 1, 0, 8, bn, split);
+        }
+        if (a.M <= bn) break;
+    }
+    pl.kblocks = (int)kb;
+    pl.tiles_p = (int)(pl.narrow ? n128 : div(a.M, pl.pair ? 256 : 128));
+    pl.tiles_q = (int)div(pl.narrow ? a.M : a.N, pl.bn);
     pl.group = pl.tiles_p < 16 ? pl.tiles_p : 16;
-    pl.extra_bytes = pl.narrow ? (pl.split > 1 ? (pl.bn + pl.split) * kXchPitch * 4 : 0) : kEpiWarps * kStageBytes + 2 * 512 * 4;
+    // no more accumulators than a CTA has units: the fewer share the epilogue warps
+    const int64_t each = div((int64_t)pl.tiles_p * pl.tiles_q, pl.pair ? sms / 2 : sms);
+    pl.bufs = pl.narrow ? 2 : 512 / pl.bn < pl.epi / 4 ? 512 / pl.bn : pl.epi / 4;
+    while (!pl.narrow && pl.bufs > 1 && pl.bufs / 2 >= each) pl.bufs /= 2;
+    pl.extra_bytes = !pl.narrow ? pl.epi * 32 * row_bytes(pl.epi) + kScaleBytes : pl.split > 1 ? (pl.bn + pl.split) * kXchPitch * 4 : 0;
     pl.extra_bytes = (pl.extra_bytes + 15) & ~15;
     const int room = kSmemCap - 1024 - pl.extra_bytes - (int)sizeof(I8Shared);
-    pl.stages = room / (kPBytes + pl.bn * kBlockK);
+    pl.stages = room / (kPBytes + pl.bn / (pl.pair ? 2 : 1) * kBlockK);
     if (pl.stages > kRingStages) pl.stages = kRingStages;
     return pl;
 }
 
-template <class T, bool NARROW>
+template <class T, bool NARROW, int CG, int EPI>
 cudaError_t launch(const I8Args &a, const I8Plan &pl, const CUtensorMap &tp, const CUtensorMap &tq, int sms, cudaStream_t st) {
-    auto k = i8_tc_kernel<T, NARROW>;
+    auto k = i8_tc_kernel<T, NARROW, CG, EPI>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap);
     if (e != cudaSuccess) return e;
     const int64_t units = (int64_t)pl.tiles_p * pl.tiles_q;
+    const int cluster = CG == 2 ? 2 : pl.split;
     cudaLaunchConfig_t cfg = {};
-    // a split unit has a cluster of its own; else persistent CTAs walk the units
-    cfg.gridDim = dim3((unsigned)(pl.split > 1 ? units * pl.split : units < sms ? units : sms));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = 1024 + (size_t)pl.stages * (kPBytes + pl.bn * kBlockK) + pl.extra_bytes + sizeof(I8Shared);
+    // a split unit has a cluster of its own; else persistent CTAs (or pairs of them) walk the units
+    cfg.gridDim = dim3((unsigned)((pl.split > 1 || units < sms / CG ? units : sms / CG) * cluster));
+    cfg.blockDim = dim3((kFirstEpi + EPI) * 32);
+    cfg.dynamicSmemBytes = 1024 + (size_t)pl.stages * (kPBytes + pl.bn / CG * kBlockK) + pl.extra_bytes + sizeof(I8Shared);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     int n = 0;
@@ -434,15 +599,22 @@ cudaError_t launch(const I8Args &a, const I8Plan &pl, const CUtensorMap &tp, con
         at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[n++].val.programmaticStreamSerializationAllowed = 1;
     }
-    if (pl.split > 1) {
+    if (cluster > 1) {
         at[n].id = cudaLaunchAttributeClusterDimension;
-        at[n].val.clusterDim.x = pl.split;
+        at[n].val.clusterDim.x = cluster;
         at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
         n++;
     }
     cfg.attrs = at;
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, k, tp, tq, a, pl);
+}
+
+template <class T>
+cudaError_t launch_form(const I8Args &a, const I8Plan &pl, const CUtensorMap &tp, const CUtensorMap &tq, int sms, cudaStream_t st) {
+    if (pl.narrow) return launch<T, true, 1, 8>(a, pl, tp, tq, sms, st);
+    if (pl.pair) return pl.epi == 16 ? launch<T, false, 2, 16>(a, pl, tp, tq, sms, st) : launch<T, false, 2, 8>(a, pl, tp, tq, sms, st);
+    return pl.epi == 16 ? launch<T, false, 1, 16>(a, pl, tp, tq, sms, st) : launch<T, false, 1, 8>(a, pl, tp, tq, sms, st);
 }
 
 }  // namespace
@@ -456,15 +628,14 @@ int i8_tc_launch(const I8Args &a, cudaStream_t st, std::string &err) {
     const int64_t units = (int64_t)pl.tiles_p * pl.tiles_q;
     if (units > (1 << 30)) { err = "too many tiles"; return -1; }
     CUtensorMap tx, tw;
-    if (!tma_encode_i8(&tx, a.x, a.K, a.M, a.ldx, pl.narrow ? pl.bn : 128, err) ||
-        !tma_encode_i8(&tw, a.w, a.K, a.N, a.ldw, pl.narrow ? 128 : pl.bn, err))
+    const int q_box = pl.bn / (pl.pair ? 2 : 1);
+    if (!tma_encode_i8(&tx, a.x, a.K, a.M, a.ldx, pl.narrow ? q_box : 128, err) ||
+        !tma_encode_i8(&tw, a.w, a.K, a.N, a.ldw, pl.narrow ? 128 : q_box, err))
         return -1;
     const CUtensorMap &tp = pl.narrow ? tw : tx, &tq = pl.narrow ? tx : tw;
-    const auto go = [&](auto type) {
-        using T = decltype(type);
-        return pl.narrow ? launch<T, true>(a, pl, tp, tq, sms, st) : launch<T, false>(a, pl, tp, tq, sms, st);
-    };
-    e = a.dtype == GCDR_DTYPE_F16 ? go(__half()) : a.dtype == GCDR_DTYPE_BF16 ? go(__nv_bfloat16()) : go(0.f);
+    e = a.dtype == GCDR_DTYPE_F16    ? launch_form<__half>(a, pl, tp, tq, sms, st)
+        : a.dtype == GCDR_DTYPE_BF16 ? launch_form<__nv_bfloat16>(a, pl, tp, tq, sms, st)
+                                     : launch_form<float>(a, pl, tp, tq, sms, st);
     if (e != cudaSuccess) {
         cudaGetLastError();
         err = cudaGetErrorString(e);
