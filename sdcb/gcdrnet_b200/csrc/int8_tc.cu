@@ -165,6 +165,23 @@ __device__ __forceinline__ float relu(float v) {
     return m;
 }
 
+__device__ __forceinline__ uint32_t relu2(uint32_t v, __half) {
+    const __half2 h = __hmax2_nan(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(0)));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t relu2(uint32_t v, __nv_bfloat16) {
+    const __nv_bfloat162 h = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&v), __bfloat162bfloat162(__ushort_as_bfloat16(0)));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float4 ld_shared(uint32_t p) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared(uint32_t p, const uint32_t *v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+
 // Unit u -> its P and Q tiles: `group` P tiles per Q tile, then the next Q tile.
 __device__ __forceinline__ void unit_tiles(const I8Plan &pl, int u, int &pt, int &qt) {
     const int per = pl.group * pl.tiles_q;
@@ -392,15 +409,19 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                 constexpr int E = 16 / (int)sizeof(T);        // elements of a 16-byte piece
                 constexpr int RB = row_bytes(EPI), PC = RB / 16;   // bytes and pieces of a stage's row
                 constexpr int CW = PC * E, LW = CW < 32 ? CW : 32;  // its columns, those of one TMEM load
-                // pieces are stored crosswise: neither the writes (a row a lane) nor the reads (a row per PC
-                // lanes) meet in a bank
-                const auto piece = [](int r, int k) { return r * RB + ((k ^ (PC == 8 ? r & 7 : (r >> 1) & 3)) * 16); };
-                uint8_t *stg = extra + e * 32 * RB;
-                T *out = static_cast<T *>(a.out);
-                const bool vec = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(a.ldo * (int64_t)sizeof(T))) & 15) == 0;
-                const int64_t mb = m0 + quad * 32;
+                constexpr int RI = 32 / PC;                   // rows of one store instruction
+                // Piece k of row r lies at r * RB + (k ^ x(r)) * 16, x = r % 8 or r / 2 % 4: neither the writes (a row a
+                // lane) nor the reads (a row per PC lanes) meet in a bank.  The same x in every RI-th row but for its
+                // highest bit (PC 8).
+                const uint32_t stg = smem_u32(extra) + (uint32_t)(e * 32 * RB);
+                const uint32_t put = stg + (uint32_t)(lane * RB + (PC == 8 ? lane & 7 : (lane >> 1) & 3) * 16);
+                const uint32_t take = stg + (uint32_t)(lane / PC * RB + (lane % PC ^ (lane >> 3)) * 16);
+                const int64_t mb = m0 + quad * 32, left = a.M - mb - lane / PC, step8 = RI * a.ldo;
+                T *out = static_cast<T *>(a.out) + (mb + lane / PC) * a.ldo + n0 + lane % PC * E;
+                const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * (int64_t)sizeof(T))) & 15) == 0;
                 const float2 rs2 = make_float2(row_s, row_s);
                 const int c_end = a.N - n0 < bn ? (int)(a.N - n0) : bn;
+                const uint32_t scale = smem_u32(sc);
                 for (int c0 = part * CW; c0 < c_end; c0 += parts * CW) {
 #pragma unroll
                     for (int h = 0; h < CW / LW; h++) {
@@ -409,54 +430,52 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                         if constexpr (LW == 32) ld.load32_nw(r);
                         else ld.load16_nw(r);
                         TmemLoader::wait_ld();
-                        const float4 *ws = reinterpret_cast<const float4 *>(sc + c0 + LW * h), *bs = ws + bn / 4;
+                        const uint32_t ws = scale + (uint32_t)(c0 + LW * h) * 4u, bs = ws + (uint32_t)bn * 4u;
 #pragma unroll
                         for (int k = 0; k < LW / E; k++) {
                             uint32_t p[4];
 #pragma unroll
                             for (int i = 0; i < E / 4; i++) {
-                                const float4 w = ws[k * (E / 4) + i], c = bs[k * (E / 4) + i];
+                                const float4 w = ld_shared(ws + (uint32_t)(k * E + 4 * i) * 4u), c = ld_shared(bs + (uint32_t)(k * E + 4 * i) * 4u);
                                 const int *q = reinterpret_cast<const int *>(r) + k * E + 4 * i;
-                                float2 v0 = __ffma2_rn(__fmul2_rn(make_float2((float)q[0], (float)q[1]), rs2), make_float2(w.x, w.y), make_float2(c.x, c.y));
-                                float2 v1 = __ffma2_rn(__fmul2_rn(make_float2((float)q[2], (float)q[3]), rs2), make_float2(w.z, w.w), make_float2(c.z, c.w));
-                                if (a.relu) {
-                                    v0 = make_float2(relu(v0.x), relu(v0.y));
-                                    v1 = make_float2(relu(v1.x), relu(v1.y));
-                                }
+                                const float2 v0 = __ffma2_rn(__fmul2_rn(make_float2((float)q[0], (float)q[1]), rs2), make_float2(w.x, w.y), make_float2(c.x, c.y));
+                                const float2 v1 = __ffma2_rn(__fmul2_rn(make_float2((float)q[2], (float)q[3]), rs2), make_float2(w.z, w.w), make_float2(c.z, c.w));
                                 if constexpr (sizeof(T) == 4) {
-                                    p[0] = __float_as_uint(v0.x); p[1] = __float_as_uint(v0.y);
-                                    p[2] = __float_as_uint(v1.x); p[3] = __float_as_uint(v1.y);
+                                    p[0] = __float_as_uint(a.relu ? relu(v0.x) : v0.x);
+                                    p[1] = __float_as_uint(a.relu ? relu(v0.y) : v0.y);
+                                    p[2] = __float_as_uint(a.relu ? relu(v1.x) : v1.x);
+                                    p[3] = __float_as_uint(a.relu ? relu(v1.y) : v1.y);
                                 } else {
                                     p[2 * i] = pack2(v0.x, v0.y, T());
                                     p[2 * i + 1] = pack2(v1.x, v1.y, T());
+                                    if (a.relu) {             // (the same once rounded)
+                                        p[2 * i] = relu2(p[2 * i], T());
+                                        p[2 * i + 1] = relu2(p[2 * i + 1], T());
+                                    }
                                 }
                             }
-                            *reinterpret_cast<uint4 *>(stg + piece(lane, h * (LW / E) + k)) = make_uint4(p[0], p[1], p[2], p[3]);
+                            st_shared(put ^ (uint32_t)((h * (LW / E) + k) * 16), p);
                         }
                     }
                     __syncwarp();
-                    const int64_t nb = n0 + c0;
-                    if (vec) {
-                        const int64_t n = nb + lane % PC * E;
+                    if (vec && (a.N % E == 0 || c0 + CW <= c_end)) {
+                        T *to = out + c0;
+                        const bool in = c0 + lane % PC * E < c_end;
 #pragma unroll
-                        for (int i = 0; i < PC; i++) {
-                            const int r = i * (32 / PC) + lane / PC;
-                            const uint8_t *from = stg + piece(r, lane % PC);
-                            if (mb + r < a.M) {
-                                T *to = out + (mb + r) * a.ldo + n;
-                                if (n + E <= a.N) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
-                                else
-                                    for (int k = 0; k < E && n + k < a.N; k++) to[k] = reinterpret_cast<const T *>(from)[k];
-                            }
+                        for (int i = 0; i < PC; i++, to += step8) {
+                            const float4 v = ld_shared((PC == 8 && (i & 1) ? take ^ 64u : take) + (uint32_t)(i * RI * RB));
+                            if (in && i * RI < left) *reinterpret_cast<float4 *>(to) = v;
                         }
                     } else {
-                        // results at odd places: an element a lane, whole rows or two of them at a time
-                        constexpr int CL = CW < 32 ? CW : 32, RI = 32 / CL;
-                        for (int r = lane / CL; r < 32 && mb + r < a.M; r += RI)
-                            for (int c = lane % CL; c < CW; c += CL)
-                                if (nb + c < a.N)
-                                    out[(mb + r) * a.ldo + nb + c] =
-                                        *reinterpret_cast<const T *>(stg + piece(r, c / E) + (c % E) * sizeof(T));
+                        // results at odd places, or a row's last piece cut short: an element a lane, whole rows or two
+                        // of them at a time
+                        constexpr int CL = CW < 32 ? CW : 32, RO = 32 / CL;
+                        T *to = static_cast<T *>(a.out) + mb * a.ldo + n0 + c0;
+                        for (int r = lane / CL; r < 32 && mb + r < a.M; r += RO)
+                            for (int c = lane % CL; c0 + c < c_end && c < CW; c += CL) {
+                                const uint32_t x = PC == 8 ? r & 7 : (r >> 1) & 3;
+                                to[r * a.ldo + c] = *reinterpret_cast<const T *>(extra + e * 32 * RB + r * RB + ((c / E) ^ x) * 16 + (c % E) * sizeof(T));
+                            }
                     }
                     __syncwarp();
                 }
@@ -522,14 +541,15 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
 
 // Picks form and tile by an estimate in SM cycles, fitted to measured sweeps (B200, K 256 to 8192, 16 to 57600
 // tokens, 160 to 8192 channels; within 15 % of the best form there):
-//   a k-block step     its bytes at 50 per cycle (what an SM draws from L2), 600 at least; 680 for a pair
-//   a unit's results   at 8 bytes per cycle with 8 epilogue warps (64-byte stores), 13 with 16 of them or when the 8 share
-//                      a single unit; 16 warps start 1500 cycles later
-//   a round            400 between units; the last one's results and the start are not hidden
+//   a k-block step     its bytes at 50 per cycle (what an SM draws from L2), 600 at least; 680 for a pair; 16 epilogue
+//                      warps leave the widest tile a ring stage less
+//   a unit's results   at 12 bytes per cycle with 8 epilogue warps (64-byte stores), 16 with 16 of them
+//   a round            700 between units; the last one's results and the start are not hidden
 //   a split of K       the join's words through distributed shared memory; clusters of eight fit the GPU 12 times
-// E.g. 57600 x 256 x 256 fp16: wide 128, 16 warps 15.6 us, 8 warps 17.5, wide 256 16.6, pair 18.5; 1800 x 512 x 512: wide
-// 64 4.6 us, 128 5.2, 16 warps 6.2; 4096^3: pair 52 us, wide 256 63, wide 128 79; 128 x 1024 x 8192: narrow 32 split 4
-// 10.9 us, wide 64 22; 16 x 2048 x 2048: split 4 6.4 us, 2 7.6, none 7.9.
+// E.g. 57600 x 256 x 256 fp16: wide 128, 16 warps 12.5 us, 8 warps 14.9, wide 256 13.4; 57600 x 512 x 512: wide 256, 16
+// warps 23.0 us, 8 warps 27.2, wide 128 26.4; 1800 x 512 x 512: wide 64 4.4 us, 128 5.0; 4096^3: pair 50 to 57 us, wide
+// 256 61, wide 128 84; 128 x 1024 x 8192: narrow 32 split 4 10.9 us, wide 64 22; 16 x 2048 x 2048: split 4 6.4 us, 2 7.6,
+// none 7.9.
 I8Plan plan_for(const I8Args &a, int sms) {
     const auto div = [](int64_t v, int64_t d) { return (v + d - 1) / d; };
     const int64_t kb = div(a.K, kBlockK);
@@ -548,11 +568,11 @@ I8Plan plan_for(const I8Args &a, int sms) {
     const int64_t m128 = div(a.M, 128);
     for (int bn = 64; bn <= 256; bn *= 2) {
         const int64_t tq = div(a.N, bn), units = m128 * tq, rounds = div(units, sms);
-        const int64_t work = kb * (bn == 256 ? 983 : bn == 128 ? 655 : 600), bytes = 128ll * bn * size;
-        const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 400) + (w > e ? e : w); };
-        offer(cost(rounds, work, rounds == 1 ? bytes / 13 : bytes / 8) + 1500, 0, 0, 8, bn, 1);
-        if (rounds > 2) offer(cost(rounds, work, bytes / 13) + 3000, 0, 0, 16, bn, 1);
-        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * 680, bytes / 8) + 5500, 0, 1, 8, bn, 1);
+        const int64_t work = kb * (bn == 256 ? 983 : bn == 128 ? 655 : 600), bytes = 128ll * (a.N < bn ? a.N : bn) * size;
+        const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 700) + (w > e ? e : w); };
+        offer(cost(rounds, work, bytes / 12) + 1500, 0, 0, 8, bn, 1);
+        if (rounds > 2) offer(cost(rounds, bn == 256 ? work * 11 / 10 : work, bytes / 16) + 2000, 0, 0, 16, bn, 1);
+        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * 680, bytes / 12) + 5500, 0, 1, 8, bn, 1);
         if (a.N <= bn) break;
     }
     const int64_t n128 = div(a.N, 128);
