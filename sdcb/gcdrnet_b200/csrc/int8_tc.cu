@@ -69,6 +69,16 @@ struct I8Shared {
     int issued, consumed;
 };
 
+// One lane of the (converged) warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -249,7 +259,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
     pdl_wait();
 
     if (warp == 0) {
-        if (lane == 0 && !a.timeout_probe) {   // (the probe issues nothing: the other roles' waits run out)
+        if (elect_one() && !a.timeout_probe) {   // (the probe issues nothing: the other roles' waits run out)
             int s = 0, issued = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
             sh->issued = issued;
         }
     } else if (warp == 1) {
-        if (lane == 0 && (CG == 1 || rank == 0)) {
+        if (elect_one() && (CG == 1 || rank == 0)) {
             const uint64_t desc0 = sdesc(0, 8 * kBlockK, 2);
             const uint32_t idesc = idesc_i8(128 * CG, bn);
             int s = 0, ab = 0, consumed = 0;
@@ -541,15 +551,15 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
 
 // Picks form and tile by an estimate in SM cycles, fitted to measured sweeps (B200, K 256 to 8192, 16 to 57600
 // tokens, 160 to 8192 channels; within 15 % of the best form there):
-//   a k-block step     its bytes at 50 per cycle (what an SM draws from L2), 600 at least; 680 for a pair; 16 epilogue
-//                      warps leave the widest tile a ring stage less
+//   a k-block step     what its loads and MMAs take together (a pair's for twice the rows); 16 epilogue warps leave
+//                      the widest tile a ring stage less
 //   a unit's results   at 12 bytes per cycle with 8 epilogue warps (64-byte stores), 16 with 16 of them
-//   a round            700 between units; the last one's results and the start are not hidden
+//   a round            700 between units; the last one's results and the start are not hidden (nor, of two units, the
+//                      second half of the warps)
 //   a split of K       the join's words through distributed shared memory; clusters of eight fit the GPU 12 times
-// E.g. 57600 x 256 x 256 fp16: wide 128, 16 warps 12.5 us, 8 warps 14.9, wide 256 13.4; 57600 x 512 x 512: wide 256, 16
-// warps 23.0 us, 8 warps 27.2, wide 128 26.4; 1800 x 512 x 512: wide 64 4.4 us, 128 5.0; 4096^3: pair 50 to 57 us, wide
-// 256 61, wide 128 84; 128 x 1024 x 8192: narrow 32 split 4 10.9 us, wide 64 22; 16 x 2048 x 2048: split 4 6.4 us, 2 7.6,
-// none 7.9.
+// E.g. 57600 x 256 x 256 fp16: wide 128, 16 warps 11.7 us, 8 warps 14.5, wide 256 13.0; 1213 x 1040 x 1000 fp32: wide 128
+// 7.4 us, 64 8.8, 256 10.5; 128 x 8192 x 8192: wide 64 16.9 us, 128 20.1; 4096^3: pair 48 us, wide 256 53, 128 56;
+// 128 x 1024 x 8192: narrow 32 split 4 9.0 us, wide 64 11.1; 16 x 1024 x 8192: split 8 6.4 us, 4 7.1, 2 9.3, none 11.3.
 I8Plan plan_for(const I8Args &a, int sms) {
     const auto div = [](int64_t v, int64_t d) { return (v + d - 1) / d; };
     const int64_t kb = div(a.K, kBlockK);
@@ -568,19 +578,19 @@ I8Plan plan_for(const I8Args &a, int sms) {
     const int64_t m128 = div(a.M, 128);
     for (int bn = 64; bn <= 256; bn *= 2) {
         const int64_t tq = div(a.N, bn), units = m128 * tq, rounds = div(units, sms);
-        const int64_t work = kb * (bn == 256 ? 983 : bn == 128 ? 655 : 600), bytes = 128ll * (a.N < bn ? a.N : bn) * size;
-        const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 700) + (w > e ? e : w); };
+        const int64_t work = kb * (bn == 256 ? 740 : bn == 128 ? 430 : 300), bytes = 128ll * (a.N < bn ? a.N : bn) * size;
+        const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 700) + (w > e ? e : w) + (r == 2 ? e : 0); };
         offer(cost(rounds, work, bytes / 12) + 1500, 0, 0, 8, bn, 1);
         if (rounds > 2) offer(cost(rounds, bn == 256 ? work * 11 / 10 : work, bytes / 16) + 2000, 0, 0, 16, bn, 1);
-        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * 680, bytes / 12) + 5500, 0, 1, 8, bn, 1);
+        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * 650, bytes / 12) + 5500, 0, 1, 8, bn, 1);
         if (a.N <= bn) break;
     }
     const int64_t n128 = div(a.N, 128);
     for (int bn = 16; a.M <= 512 && bn <= 128; bn *= 2) {
-        const int64_t tiles = n128 * div(a.M, bn), step = bn == 128 ? 655 : 600;
+        const int64_t tiles = n128 * div(a.M, bn), step = bn == 128 ? 430 : bn == 64 ? 330 : 270;
         for (int split = 1; split <= 8 && split <= kb; split *= 2) {
             const int64_t rounds = div(tiles * split, split == 8 ? 96 : sms);
-            offer(rounds * (div(kb, split) * step + (split > 1 ? 1500 + bn * 100 : 0)) + 4000 + bn * 30, 1, 0, 8, bn, split);
+            offer(rounds * (div(kb, split) * step + (split > 1 ? 1500 + bn * 100 : 0)) + 3300 + bn * 30, 1, 0, 8, bn, split);
         }
         if (a.M <= bn) break;
     }
