@@ -395,7 +395,8 @@ GCDR_API int gcdr_k_quant_rows(const void *x, int dtype, int64_t rows, int C, in
 /* out[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], then relu (a NaN stays NaN), rounded to
  * `dtype`.  The integer sum is exact: K 1..131071 (int32 sums of products up to 2^14).
  *   x    int8 [M][K], pitch ldx, xs M scales;   w  int8 [N][K], pitch ldw, ws N scales
- *        x and w 16-byte aligned, ldx and ldw multiples of 16 (K and N are free)
+ *        x and w 16-byte aligned, ldx and ldw multiples of 16 (K and N are free); rows on
+ *        128-byte lines (ldx, ldw multiples of 128) read up to twice as fast
  *   bias N floats or NULL
  *   wait_cycles, timeout_probe: as in gcdr_conv_desc (gcdr_k_status reports a wait that ran out) */
 typedef struct {

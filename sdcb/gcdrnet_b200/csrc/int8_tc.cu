@@ -192,6 +192,25 @@ __device__ __forceinline__ void st_shared(uint32_t p, const uint32_t *v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 
+// A store stage's rows of RB bytes to rows at any element, V at a time
+template <class V, int RB, class T>
+__device__ __forceinline__ void store_rows(const uint8_t *from, T *to, int64_t ldo, int rows, int cols, int lane) {
+    constexpr int E = sizeof(V) / sizeof(T), LR = RB / (int)sizeof(V), CL = LR < 32 ? LR : 32, RO = 32 / CL, PC = RB / 16;
+#pragma unroll 4
+    for (int r = lane / CL; r < rows; r += RO) {
+        const int x = PC == 8 ? r & 7 : (r >> 1) & 3;
+#pragma unroll
+        for (int i = 0; i < LR / CL; i++) {
+            const int c = lane % CL + i * CL, byte = c * (int)sizeof(V);
+            const uint8_t *p = from + r * RB + (((byte >> 4) ^ x) << 4) + (byte & 15);
+            T *q = to + r * ldo + c * E;
+            if ((c + 1) * E <= cols) *reinterpret_cast<V *>(q) = *reinterpret_cast<const V *>(p);
+            else
+                for (int k = 0; c * E + k < cols; k++) q[k] = reinterpret_cast<const T *>(p)[k];
+        }
+    }
+}
+
 // Unit u -> its P and Q tiles: `group` P tiles per Q tile, then the next Q tile.
 __device__ __forceinline__ void unit_tiles(const I8Plan &pl, int u, int &pt, int &qt) {
     const int per = pl.group * pl.tiles_q;
@@ -477,15 +496,14 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                             if (in && i * RI < left) *reinterpret_cast<float4 *>(to) = v;
                         }
                     } else {
-                        // results at odd places, or a row's last piece cut short: an element a lane, whole rows or two
-                        // of them at a time
-                        constexpr int CL = CW < 32 ? CW : 32, RO = 32 / CL;
+                        // results at odd places, or a row's last piece cut short
+                        const unsigned odd = (unsigned)(reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * (int64_t)sizeof(T))) & 15u;
+                        const uint8_t *from = extra + e * 32 * RB;
                         T *to = static_cast<T *>(a.out) + mb * a.ldo + n0 + c0;
-                        for (int r = lane / CL; r < 32 && mb + r < a.M; r += RO)
-                            for (int c = lane % CL; c0 + c < c_end && c < CW; c += CL) {
-                                const uint32_t x = PC == 8 ? r & 7 : (r >> 1) & 3;
-                                to[r * a.ldo + c] = *reinterpret_cast<const T *>(extra + e * 32 * RB + r * RB + ((c / E) ^ x) * 16 + (c % E) * sizeof(T));
-                            }
+                        const int rows = a.M - mb < 32 ? (int)(a.M - mb) : 32, cols = c_end - c0;
+                        if (odd % 8 == 0) store_rows<uint2, RB>(from, to, a.ldo, rows, cols, lane);
+                        else if (sizeof(T) == 4 || odd % 4 == 0) store_rows<uint32_t, RB>(from, to, a.ldo, rows, cols, lane);
+                        else store_rows<T, RB>(from, to, a.ldo, rows, cols, lane);
                     }
                     __syncwarp();
                 }
@@ -551,8 +569,9 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
 
 // Picks form and tile by an estimate in SM cycles, fitted to measured sweeps (B200, K 256 to 8192, 16 to 57600
 // tokens, 160 to 8192 channels; within 15 % of the best form there):
-//   a k-block step     what its loads and MMAs take together (a pair's for twice the rows); 16 epilogue warps leave
-//                      the widest tile a ring stage less
+//   a k-block step     what its loads and MMAs take together (a pair's for twice the rows; the second figures where
+//                      rows do not start on a line: each 128 bytes are then two requests); 16 epilogue warps leave a
+//                      ring stage less
 //   a unit's results   at 12 bytes per cycle with 8 epilogue warps (64-byte stores), 16 with 16 of them
 //   a round            700 between units; the last one's results and the start are not hidden (nor, of two units, the
 //                      second half of the warps)
@@ -575,22 +594,23 @@ I8Plan plan_for(const I8Args &a, int sms) {
         pl.bn = bn;
         pl.split = split;
     };
+    const bool cut = (a.ldx | a.ldw) % 128 != 0;   // a box's 128 bytes lie in two lines each
     const int64_t m128 = div(a.M, 128);
     for (int bn = 64; bn <= 256; bn *= 2) {
         const int64_t tq = div(a.N, bn), units = m128 * tq, rounds = div(units, sms);
-        const int64_t work = kb * (bn == 256 ? 740 : bn == 128 ? 430 : 300), bytes = 128ll * (a.N < bn ? a.N : bn) * size;
+        const int64_t work = kb * (cut ? (bn == 256 ? 1300 : bn == 128 ? 950 : 670) : bn == 256 ? 740 : bn == 128 ? 430 : 300), bytes = 128ll * (a.N < bn ? a.N : bn) * size;
         const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 700) + (w > e ? e : w) + (r == 2 ? e : 0); };
         offer(cost(rounds, work, bytes / 12) + 1500, 0, 0, 8, bn, 1);
-        if (rounds > 2) offer(cost(rounds, bn == 256 ? work * 11 / 10 : work, bytes / 16) + 2000, 0, 0, 16, bn, 1);
-        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * 650, bytes / 12) + 5500, 0, 1, 8, bn, 1);
+        if (rounds > 2) offer(cost(rounds, work * 11 / 10, bytes / 16) + 2000, 0, 0, 16, bn, 1);
+        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * (cut ? 1000 : 650), bytes / 12) + 5500, 0, 1, 8, bn, 1);
         if (a.N <= bn) break;
     }
     const int64_t n128 = div(a.N, 128);
     for (int bn = 16; a.M <= 512 && bn <= 128; bn *= 2) {
-        const int64_t tiles = n128 * div(a.M, bn), step = bn == 128 ? 430 : bn == 64 ? 330 : 270;
+        const int64_t tiles = n128 * div(a.M, bn), step = (bn == 128 ? 430 : bn == 64 ? 330 : 270) * (cut ? 2 : 1);
         for (int split = 1; split <= 8 && split <= kb; split *= 2) {
             const int64_t rounds = div(tiles * split, split == 8 ? 96 : sms);
-            offer(rounds * (div(kb, split) * step + (split > 1 ? 1500 + bn * 100 : 0)) + 3300 + bn * 30, 1, 0, 8, bn, split);
+            offer(rounds * (div(kb, split) * step + (split > 1 ? 1500 + bn * 100 : 0)) + 3300 + bn * 50, 1, 0, 8, bn, split);
         }
         if (a.M <= bn) break;
     }

@@ -202,14 +202,6 @@ struct RowMath {
     __device__ __forceinline__ RowMath(const RowArgs &a_, float *slots, int l)
         : a(a_), grp{slots}, first(l * Part::P), left(a_.C - l * Part::P), g1(at(a_.g1)), b1(at(a_.b1)), g2(at(a_.g2)), b2(at(a_.b2)) {}
     __device__ __forceinline__ const float *at(const float *p) const { return p ? p + first : p; }
-    __device__ __forceinline__ void gain4(const float *p, int k, float2 *v) const {
-        if (p) Part::param4(p, left, k, 1.f, v);
-        else v[0] = v[1] = both(1.f);
-    }
-    __device__ __forceinline__ void shift4(const float *p, int k, float2 *v) const {
-        if (p) Part::param4(p, left, k, 0.f, v);
-        else v[0] = v[1] = both(0.f);
-    }
     __device__ __forceinline__ void norm(float2 *v, int kind, const float *g, const float *b, float eps) {
         if (kind == GCDR_NORM_LAYER) {
             float2 s = both(0.f);
@@ -226,13 +218,24 @@ struct RowMath {
 #pragma unroll
         for (int i = 0; i < E / 2; i++) q = __ffma2_rn(v[i], v[i], q);
         const float2 rstd = both(inv_sqrt(fmaf(grp.sum(q.x + q.y), a.inv_C, eps)));
+        if (g && b) affine<true, true>(v, rstd, g, b);
+        else if (g) affine<true, false>(v, rstd, g, b);
+        else if (b) affine<false, true>(v, rstd, g, b);
+        else affine<false, false>(v, rstd, g, b);
+    }
+    template <bool GAIN, bool SHIFT>
+    __device__ __forceinline__ void affine(float2 *v, float2 rstd, const float *g, const float *b) const {
 #pragma unroll
         for (int k = 0; k < E / 4; k++) {
             float2 t[4];
-            gain4(g, k, t);
-            shift4(b, k, t + 2);
-            v[2 * k] = __ffma2_rn(__fmul2_rn(v[2 * k], rstd), t[0], t[2]);
-            v[2 * k + 1] = __ffma2_rn(__fmul2_rn(v[2 * k + 1], rstd), t[1], t[3]);
+            if (GAIN) Part::param4(g, left, k, 1.f, t);
+            if (SHIFT) Part::param4(b, left, k, 0.f, t + 2);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float2 &x = v[2 * k + i];
+                x = __fmul2_rn(x, rstd);
+                x = GAIN && SHIFT ? __ffma2_rn(x, t[i], t[2 + i]) : GAIN ? __fmul2_rn(x, t[i]) : SHIFT ? __fadd2_rn(x, t[2 + i]) : x;
+            }
         }
     }
 
