@@ -37,7 +37,7 @@ def untouched(view, buf, fill):
     """Nothing between the rows of `view` was written."""
     import torch
     mask = torch.ones_like(buf, dtype=torch.bool)
-    mask.as_strided(view.shape, view.stride())[:] = False
+    mask.as_strided(view.shape, view.stride(), view.storage_offset())[:] = False
     rest = buf[mask]
     return bool((rest == fill).all().item()) if rest.numel() else True
 

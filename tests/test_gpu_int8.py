@@ -139,7 +139,14 @@ PRODUCTS = [(1, 1, 1), (1, 16, 16), (1, 512, 512), (1, 1000, 4096), (2, 33, 31),
             (33, 512, 48), (50, 96, 65), (64, 256, 256), (65, 40, 513), (100, 1037, 1000), (127, 128, 128),
             (128, 128, 32), (128, 256, 256), (129, 257, 257), (200, 512, 512), (256, 256, 128), (257, 100, 1),
             (300, 16, 4096), (511, 160, 160), (1000, 300, 77), (1800, 512, 512), (2049, 513, 640), (7200, 160, 160),
-            (1, 20000, 64), (20000, 1, 64)]
+            (1, 20000, 64), (20000, 1, 64), (2, 5000, 700), (4, 4100, 2000), (1, 4097, 2049),
+            # few tokens against long rows: K split over two, four and eight CTAs
+            (20, 1000, 2000), (12, 100, 4000), (70, 1000, 16000), (33, 300, 9001), (500, 130, 16384), (40, 4096, 1024),
+            (61, 1001, 65000), (99, 4096, 16384), (250, 2047, 8190), (500, 639, 32760),
+            # units of 256 tokens over two CTAs, the last ones ragged
+            (4000, 2500, 3000), (3001, 2051, 3001), (2600, 4104, 4096),
+            # several units a CTA: two and four accumulators, groups of 4 and 8 epilogue warps
+            (20001, 300, 200), (30011, 100, 64), (40000, 160, 128), (9001, 513, 1024), (5003, 2000, 300)]
 
 
 @pytest.mark.parametrize("size", PRODUCTS, ids=lambda s: "%dx%dx%d" % s)
@@ -159,18 +166,21 @@ def test_i8_gemm_pitches(M, dtype):
     _check_product(M, 40, 33, dtype, False, ldo=41, ldx=48, ldw=64)
 
 
-@pytest.mark.parametrize("M", [1, 20, 150])
-def test_i8_gemm_unaligned_result(M):
-    """The result starts one element past any vector's border."""
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N", [(1, 64), (20, 64), (150, 136), (700, 300), (20001, 72)])
+def test_i8_gemm_result_alignments(M, N, dtype):
+    """The result's rows start 16, 8, 4 or 2 bytes off a vector's border, at pitches of every such multiple."""
     import torch
-    x, xs, w, ws, b = _operands(M, 64, 64, 3)
-    for dt in (torch.float16, torch.float32):
-        buf = torch.full((M * 64 + 2,), 9.0, dtype=dt, device="cuda:0")
-        out = buf[1:-1].view(M, 64)
+    dt = torch_dtype(dtype)
+    x, xs, w, ws, b = _operands(M, N, 64, 3)
+    want, bound = ref_product(x, xs, w, ws, b, False, dt)
+    for off, more in ((1, 0), (2, 0), (4, 8), (0, 2), (0, 4), (0, 1), (3, 5)):
+        ldo = N + more
+        buf = torch.full(((M - 1) * ldo + N + off + 1,), 9.0, dtype=dt, device="cuda:0")
+        out = buf[off:].as_strided((M, N), (ldo, 1))
         assert i8_gemm(x, xs, w, ws, b, out) == 0
-        want, bound = ref_product(x, xs, w, ws, b, False, dt)
-        assert worst(out, want, bound) <= 1.0
-        assert buf[0] == 9.0 and buf[-1] == 9.0
+        assert worst(out, want, bound) <= 1.0, (off, more)
+        assert untouched(out, buf, 9.0), (off, more)
 
 
 @pytest.mark.parametrize("M,N", [(1, 40), (24, 70), (200, 130)])
