@@ -379,10 +379,11 @@ cudaError_t launch_rows(const RowArgs &a, bool vec, cudaStream_t st) {
 
 }  // namespace
 
-// G and NCH by the row's length: 16 elements a thread, 24 where that leaves fewer threads idle (1037 fp32 elements in
-// 64 x 24 instead of 128 x 16: 4.7 against 5.7 us for 4099 rows), up to the 256 threads whose reductions cost least
-// (4096 bf16, both norms, 16384 rows: 256 x 16 102 us, 512 x 16 226 us, 512 x 8 134 us; 8192: 256 x 32 101 us, 512 x 16
-// 124 us for the norms, 81 against 72 us for the rounding alone, which needs few registers).
+// G and NCH by the row's length: 16 elements a thread, 24 where that leaves fewer threads idle (4099 rows of 1037 fp32
+// elements to int8: 64 x 24 4.7 us, 128 x 16 5.7).  The norms of long 16-bit rows, whose instructions and reductions bound
+// them, take 32 in half the threads (16384 rows of 4096 bf16, both RMS: 128 x 32 92 us, 256 x 16 106, 512 x 8 134; both
+// LayerNorm 126 against 143; 8192 rows of 2048, LayerNorm, 58 against 64); fp32 rows, bound by their bytes, do not (94 us
+// against 96).
 template <class T, bool QUANT>
 cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st) {
     const int C = a.C;
@@ -395,11 +396,12 @@ cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st) {
     if (C <= 768) return launch_rows<T, 32, 3, QUANT>(a, vec, st);
     if (C <= 1024) return launch_rows<T, 64, 2, QUANT>(a, vec, st);
     if (C <= 1536) return launch_rows<T, 64, 3, QUANT>(a, vec, st);
-    if (C <= 2048) return launch_rows<T, 128, 2, QUANT>(a, vec, st);
+    constexpr bool LONG = !QUANT && sizeof(T) == 2;
+    if (C <= 2048) return launch_rows<T, LONG ? 64 : 128, LONG ? 4 : 2, QUANT>(a, vec, st);
     if (C <= (3 << 10)) return launch_rows<T, 128, 3, QUANT>(a, vec, st);
-    if (C <= 4096) return launch_rows<T, 256, 2, QUANT>(a, vec, st);
+    if (C <= 4096) return launch_rows<T, LONG ? 128 : 256, LONG ? 4 : 2, QUANT>(a, vec, st);
     if (C <= 6144) return launch_rows<T, 256, 3, QUANT>(a, vec, st);
-    if (C <= 8192) return launch_rows<T, QUANT ? 512 : 256, QUANT ? 2 : 4, QUANT>(a, vec, st);
+    if (C <= 8192) return launch_rows<T, 512, 2, QUANT>(a, vec, st);
     if (C <= 16384) return launch_rows<T, 1024, 2, QUANT>(a, vec, st);
     return launch_rows<T, 1024, 4, QUANT>(a, vec, st);
 }
