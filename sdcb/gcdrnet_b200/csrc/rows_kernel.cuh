@@ -185,6 +185,19 @@ struct RowPart {
             }
         }
     }
+    // the same from a table in shared memory that fills the whole group
+    static __device__ __forceinline__ void table4(uint32_t p, int k, float2 *v) {
+        if constexpr (VEC) {
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y) : "r"(p + 4u * at(4 * k)) : "memory");
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float t;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(t) : "r"(p + 4u * at(4 * k + e)) : "memory");
+                (e & 1 ? v[e / 2].y : v[e / 2].x) = t;
+            }
+        }
+    }
 };
 
 // The arithmetic of a row once its group holds it: 8 * NCH elements a thread, zeros past its end (and zeros they
@@ -194,6 +207,12 @@ struct RowMath {
     using Part = RowPart<T, G, NCH, FIT>;
     static constexpr bool VEC = FIT != kOdd;
     static constexpr int E = 8 * NCH;
+    // 16-bit rows of a warp or less keep the gains and shifts in shared memory, 1 and 0 past the row and where there
+    // are none (57600 rows of 256 fp16, both norms, to int8: 28 us against 31 from L1, which the rows pass through; fp32
+    // rows, bound by their bytes, lose 3 % by it).
+    static constexpr bool TABLE = G <= 32 && !QUANT && sizeof(T) == 2;
+    static constexpr int W = G * E;         // floats of one of its four rows: g1, b1, g2, b2
+    uint32_t table = 0;                     // this thread's first element of g1
     const RowArgs &a;
     Group<G> grp;
     const int first, left;                  // this thread's first element, and how many the row has from there
@@ -202,7 +221,10 @@ struct RowMath {
     __device__ __forceinline__ RowMath(const RowArgs &a_, float *slots, int l)
         : a(a_), grp{slots}, first(l * Part::P), left(a_.C - l * Part::P), g1(at(a_.g1)), b1(at(a_.b1)), g2(at(a_.g2)), b2(at(a_.b2)) {}
     __device__ __forceinline__ const float *at(const float *p) const { return p ? p + first : p; }
-    __device__ __forceinline__ void norm(float2 *v, int kind, const float *g, const float *b, float eps) {
+    __device__ __forceinline__ void norm(float2 *v, bool second) {
+        const int kind = second ? a.pre : a.post;
+        const float *g = second ? g2 : g1, *b = second ? b2 : b1;
+        const float eps = second ? a.eps2 : a.eps1;
         if (kind == GCDR_NORM_LAYER) {
             float2 s = both(0.f);
 #pragma unroll
@@ -218,10 +240,41 @@ struct RowMath {
 #pragma unroll
         for (int i = 0; i < E / 2; i++) q = __ffma2_rn(v[i], v[i], q);
         const float2 rstd = both(inv_sqrt(fmaf(grp.sum(q.x + q.y), a.inv_C, eps)));
+        if constexpr (TABLE) {
+            const uint32_t t = table + (second ? 8u * W : 0u);
+            if (b) from_table<true>(v, rstd, t);
+            else from_table<false>(v, rstd, t);
+            return;
+        }
         if (g && b) affine<true, true>(v, rstd, g, b);
         else if (g) affine<true, false>(v, rstd, g, b);
         else if (b) affine<false, true>(v, rstd, g, b);
         else affine<false, false>(v, rstd, g, b);
+    }
+    template <bool SHIFT>
+    __device__ __forceinline__ void from_table(float2 *v, float2 rstd, uint32_t p) const {
+#pragma unroll
+        for (int k = 0; k < E / 4; k++) {
+            float2 g[2], b[2];
+            Part::table4(p, k, g);
+            if (SHIFT) Part::table4(p + 4u * W, k, b);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float2 &x = v[2 * k + i];
+                x = __fmul2_rn(x, rstd);
+                x = SHIFT ? __ffma2_rn(x, g[i], b[i]) : __fmul2_rn(x, g[i]);
+            }
+        }
+    }
+    // fills the table: every thread of the block, before the first norm
+    __device__ __forceinline__ void fill(float *t) {
+        for (int i = threadIdx.x; i < 4 * W; i += blockDim.x) {
+            const int row = i / W, c = i - row * W;
+            const float *p = row == 0 ? a.g1 : row == 1 ? a.b1 : row == 2 ? a.g2 : a.b2;
+            t[i] = p && c < a.C ? p[c] : row & 1 ? 0.f : 1.f;
+        }
+        table = (uint32_t)__cvta_generic_to_shared(t) + 4u * first;
+        __syncthreads();
     }
     template <bool GAIN, bool SHIFT>
     __device__ __forceinline__ void affine(float2 *v, float2 rstd, const float *g, const float *b) const {
@@ -241,7 +294,7 @@ struct RowMath {
 
     // v = N1(v), then v = x + res_scale * gate . v
     __device__ __forceinline__ void join(float2 *v, const Part &gate, const Part &x) {
-        if (a.post) norm(v, a.post, g1, b1, a.eps1);
+        if (a.post) norm(v, false);
         float2 t[E / 2];
         if (a.gate) {
             gate.get(t);
@@ -262,7 +315,7 @@ struct RowMath {
         const int n = left;
         if (!QUANT) {
             if (a.r && valid) Part::store(static_cast<T *>(a.r) + row * a.ldr + first, n, v);
-            if (a.pre) norm(v, a.pre, g2, b2, a.eps2);
+            if (a.pre) norm(v, true);
             if (a.y && valid) Part::store(static_cast<T *>(a.y) + row * a.ldy + first, n, v);
         }
         if (QUANT || a.q) quant(v, row, valid);
@@ -328,6 +381,10 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) rows_kernel(const __grid_con
     if (has_f) load_f(clip(base + g));
     if (has_gate) gate.load(m.gate_row(clip(base + g)), m.left);
     if (has_x) load_x(clip(base + g));
+    if constexpr (Math::TABLE) {
+        __shared__ float table[4 * Math::W];
+        m.fill(table);
+    }
     for (; base < a.rows; base += stride) {
         const int64_t row = base + g, next = clip(row + stride);
         const bool more = base + stride < a.rows;
