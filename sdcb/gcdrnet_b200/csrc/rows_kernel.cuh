@@ -362,8 +362,10 @@ struct RowMath {
     }
 };
 
+// (two registers more than four blocks of 128 threads leave would cost the longest 16-bit norms a block: 16384 rows of
+// 4096 bf16, RMS, 88.8 us against 93.0)
 template <class T, int G, int NCH, Fit FIT, bool QUANT>
-__global__ void __launch_bounds__(G > 32 ? G : 256) rows_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(G > 32 ? G : 256, G == 128 && NCH == 4 && FIT != kOdd ? 4 : 0) rows_kernel(const __grid_constant__ RowArgs a) {
     constexpr int RPB = G > 32 ? 1 : 256 / G;   // rows per block
     using Math = RowMath<T, G, NCH, FIT, QUANT>;
     __shared__ float slots[G > 32 ? 2 * (G / 32) : 1];
@@ -438,8 +440,8 @@ cudaError_t launch_rows(const RowArgs &a, bool vec, cudaStream_t st) {
 
 // G and NCH by the row's length: 16 elements a thread, 24 where that leaves fewer threads idle (4099 rows of 1037 fp32
 // elements to int8: 64 x 24 4.7 us, 128 x 16 5.7).  The norms of long 16-bit rows, whose instructions and reductions bound
-// them, take 32 in half the threads (16384 rows of 4096 bf16, both RMS: 128 x 32 92 us, 256 x 16 106, 512 x 8 134; both
-// LayerNorm 126 against 143; 8192 rows of 2048, LayerNorm, 58 against 64); fp32 rows, bound by their bytes, do not (94 us
+// them, take 32 in half the threads (16384 rows of 4096 bf16, both RMS: 128 x 32 89 us, 256 x 16 106, 512 x 8 134; both
+// LayerNorm 123 against 143; 8192 rows of 2048, LayerNorm, 58 against 64); fp32 rows, bound by their bytes, do not (94 us
 // against 96).
 template <class T, bool QUANT>
 cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st) {
