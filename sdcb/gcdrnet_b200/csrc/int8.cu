@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(128) i8_dot_kernel(const __grid_constant__ I8A
                         from_f32<T>(scaled(sum, a.xs[j], a.ws[n0 + r], a.bias ? a.bias[n0 + r] : 0.f, a.relu));
             }
     }
-    pdl_trigger();
+    pdl_trigger();   // (earlier, the next kernel's blocks wait beside these: 8192 x 8192 12.7 us against 12.0)
 }
 
 template <class T, int MT, int R, int U>

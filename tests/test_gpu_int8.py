@@ -516,6 +516,44 @@ def test_calls_are_captured_and_replayed():
                 assert torch.equal(v, s[k]), k
 
 
+def test_calls_back_to_back_on_reused_buffers():
+    """Calls that follow one another on one stream, each on buffers that the one before read or wrote (in place and
+    apart), give what the same calls give with a wait between them."""
+    import torch
+    g = _gen(77)
+    C = 256
+    w = torch.randint(-127, 128, (C, C), generator=g, device="cuda:0").to(torch.int8)
+    ws, bias = torch.rand(C, generator=g, device="cuda:0") * 2e-3, _rand(g, C, scale=0.1)
+    gain, shift = 1 + _rand(g, C, scale=0.1), _rand(g, C, scale=0.1)
+    for rows in (1, 700, 9001):
+        start = _rand(g, rows, C).half()
+
+        def chain(wait):
+            x, q, s = start.clone(), torch.zeros(rows, C, dtype=torch.int8, device="cuda:0"), torch.zeros(rows, device="cuda:0")
+            h = torch.zeros(rows, C, dtype=torch.float16, device="cuda:0")
+            torch.cuda.synchronize()
+            for _ in range(12):
+                assert block_norm(x=x, pre=LAYER, g2=gain, b2=shift, q=q, qs=s) == 0
+                if wait:
+                    torch.cuda.synchronize()
+                assert i8_gemm(q, s, w, ws, bias, h, relu=True) == 0
+                if wait:
+                    torch.cuda.synchronize()
+                assert block_norm(x=x, f=h, post=RMS, g1=gain, scale=0.5, r=x, pre=RMS, g2=gain, y=h) == 0
+                if wait:
+                    torch.cuda.synchronize()
+                assert quant_rows(h, q, s) == 0
+                assert i8_gemm(q, s, w, ws, None, h) == 0
+                assert block_norm(x=x, f=h, scale=0.1, r=x) == 0
+                if wait:
+                    torch.cuda.synchronize()
+            torch.cuda.synchronize()
+            return x, h, q, s
+
+        for got, want in zip(chain(False), chain(True)):
+            assert torch.equal(got, want)
+
+
 def test_refusals_with_device_operands():
     """Host memory, overlapping operands: refused before anything is launched."""
     import torch
