@@ -206,8 +206,12 @@ extern "C" int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream) {
                       d->wait_cycles, d->timeout_probe != 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a.M > kDotTokens || a.timeout_probe) {
-        std::string err;
-        return i8_tc_launch(a, st, err) ? refuse(who, GCDR_ERR_DEVICE, err.c_str()) : GCDR_OK;
+        try {
+            std::string err;
+            return i8_tc_launch(a, st, err) ? refuse(who, GCDR_ERR_DEVICE, err.c_str()) : GCDR_OK;
+        } catch (...) {   // (of the message's memory: nothing leaves a C entry)
+            return GCDR_ERR_OOM;
+        }
     }
     const cudaError_t e = d->dtype == GCDR_DTYPE_F16    ? launch_dot<__half>(a, st)
                           : d->dtype == GCDR_DTYPE_BF16 ? launch_dot<__nv_bfloat16>(a, st)

@@ -445,23 +445,23 @@ cudaError_t launch_rows(const RowArgs &a, bool vec, cudaStream_t st) {
 // against 96).
 template <class T, bool QUANT>
 cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st) {
-    const int C = a.C;
-    if (C <= 64) return launch_rows<T, 8, 1, QUANT>(a, vec, st);
-    if (C <= 128) return launch_rows<T, 8, 2, QUANT>(a, vec, st);
-    if (C <= 192) return launch_rows<T, 8, 3, QUANT>(a, vec, st);
-    if (C <= 256) return launch_rows<T, 16, 2, QUANT>(a, vec, st);
-    if (C <= 384) return launch_rows<T, 16, 3, QUANT>(a, vec, st);
-    if (C <= 512) return launch_rows<T, 32, 2, QUANT>(a, vec, st);
-    if (C <= 768) return launch_rows<T, 32, 3, QUANT>(a, vec, st);
-    if (C <= 1024) return launch_rows<T, 64, 2, QUANT>(a, vec, st);
-    if (C <= 1536) return launch_rows<T, 64, 3, QUANT>(a, vec, st);
+    const auto fits = [&](int g, int nch) { return a.C <= 8 * g * nch; };
     constexpr bool LONG = !QUANT && sizeof(T) == 2;
-    if (C <= 2048) return launch_rows<T, LONG ? 64 : 128, LONG ? 4 : 2, QUANT>(a, vec, st);
-    if (C <= (3 << 10)) return launch_rows<T, 128, 3, QUANT>(a, vec, st);
-    if (C <= 4096) return launch_rows<T, LONG ? 128 : 256, LONG ? 4 : 2, QUANT>(a, vec, st);
-    if (C <= 6144) return launch_rows<T, 256, 3, QUANT>(a, vec, st);
-    if (C <= 8192) return launch_rows<T, 512, 2, QUANT>(a, vec, st);
-    if (C <= 16384) return launch_rows<T, 1024, 2, QUANT>(a, vec, st);
+    if (fits(8, 1)) return launch_rows<T, 8, 1, QUANT>(a, vec, st);
+    if (fits(8, 2)) return launch_rows<T, 8, 2, QUANT>(a, vec, st);
+    if (fits(8, 3)) return launch_rows<T, 8, 3, QUANT>(a, vec, st);
+    if (fits(16, 2)) return launch_rows<T, 16, 2, QUANT>(a, vec, st);
+    if (fits(16, 3)) return launch_rows<T, 16, 3, QUANT>(a, vec, st);
+    if (fits(32, 2)) return launch_rows<T, 32, 2, QUANT>(a, vec, st);
+    if (fits(32, 3)) return launch_rows<T, 32, 3, QUANT>(a, vec, st);
+    if (fits(64, 2)) return launch_rows<T, 64, 2, QUANT>(a, vec, st);
+    if (fits(64, 3)) return launch_rows<T, 64, 3, QUANT>(a, vec, st);
+    if (fits(64, 4)) return launch_rows<T, LONG ? 64 : 128, LONG ? 4 : 2, QUANT>(a, vec, st);
+    if (fits(128, 3)) return launch_rows<T, 128, 3, QUANT>(a, vec, st);
+    if (fits(128, 4)) return launch_rows<T, LONG ? 128 : 256, LONG ? 4 : 2, QUANT>(a, vec, st);
+    if (fits(256, 3)) return launch_rows<T, 256, 3, QUANT>(a, vec, st);
+    if (fits(512, 2)) return launch_rows<T, 512, 2, QUANT>(a, vec, st);
+    if (fits(1024, 2)) return launch_rows<T, 1024, 2, QUANT>(a, vec, st);
     return launch_rows<T, 1024, 4, QUANT>(a, vec, st);
 }
 
