@@ -15,15 +15,15 @@
 //                 tokens.  (Integers: the join is exact and the same at any split.)
 //
 // 4 + EPI warps: TMA producer, MMA issuer, TMEM allocation, one idle, and the epilogue warps, which read the TMEM lane
-// quadrant of their number.  TMEM holds up to four accumulators; in the wide form each has its own group of epilogue
+// quadrant of their number.  Producer and issuer are one elected lane (elect.sync): the compiler then knows that one
+// thread is active; under a test of the lane's number a stage's two copies cost 420 cycles instead of 240 and a block's
+// four MMAs 560 instead of 260.  TMEM holds up to four accumulators; in the wide form each has its own group of epilogue
 // warps, so that several units' epilogues, whose latencies add up to more than a unit's MMAs, run side by side.
 // The tail of K and rows past an operand's end arrive as zeros (TMA fill).  Every mbarrier wait is
 // bounded, as in conv_tc.cu.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
-#include <cstdio>
 #include <string>
 
 #include "conv_launch.h"
@@ -161,11 +161,6 @@ __device__ __forceinline__ void free_tmem(uint32_t base, uint32_t cols) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
     else
         tmem_dealloc(base, cols);
-}
-
-__device__ __forceinline__ float scaled(int acc, float xs, float ws, float bias, bool relu) {
-    const float v = fmaf((float)acc * xs, ws, bias);
-    return relu && v < 0.f ? 0.f : v;   // (a NaN stays)
 }
 
 // max(v, 0), a NaN stays
@@ -430,7 +425,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                     for (int j = 0; j < 16; j++) {
                         const int64_t m = m0 + c0 + j;
                         if (m >= a.M) break;
-                        const float v = scaled((int)r[j], a.xs[m], row_s, row_b, a.relu);
+                        const float v = i8_result((int)r[j], a.xs[m], row_s, row_b, a.relu);
                         if (n0 + row < a.N) out[m * a.ldo + n0 + row] = from_f32<T>(v);
                     }
                 }
@@ -540,7 +535,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                     if (at * split + (int)rank >= bn || m >= a.M) break;
                     int sum = 0;
                     for (int r = 0; r < split; r++) sum += xch[(r * cols + at) * kXchPitch + row];
-                    static_cast<T *>(a.out)[m * a.ldo + n] = from_f32<T>(scaled(sum, a.xs[m], ws, bs, a.relu));
+                    static_cast<T *>(a.out)[m * a.ldo + n] = from_f32<T>(i8_result(sum, a.xs[m], ws, bs, a.relu));
                 }
             }
         }

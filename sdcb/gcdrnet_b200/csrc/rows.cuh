@@ -58,26 +58,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// 8 consecutive elements, 16-byte aligned
-template <class T> __device__ __forceinline__ void load8(const T *p, float *v) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    unpack2(u.x, v, T());
-    unpack2(u.y, v + 2, T());
-    unpack2(u.z, v + 4, T());
-    unpack2(u.w, v + 6, T());
-}
-template <> __device__ __forceinline__ void load8<float>(const float *p, float *v) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <class T> __device__ __forceinline__ void store8(T *p, const float *v) {
-    *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()),
-                                               pack2(v[6], v[7], T()));
-}
-template <> __device__ __forceinline__ void store8<float>(float *p, const float *v) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+// One result of the int8 product: a rounding of the sum's (up to 31) bits to fp32 and two of the scaling.  The sum
+// takes one scale, then the other: the product of the two alone could leave the normal numbers.
+__device__ __forceinline__ float i8_result(int acc, float xs, float ws, float bias, bool relu) {
+    const float v = fmaf((float)acc * xs, ws, bias);
+    return relu && v < 0.f ? 0.f : v;   // (a NaN stays)
 }
 
 }  // namespace gcdr

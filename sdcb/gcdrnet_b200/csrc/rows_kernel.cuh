@@ -104,23 +104,23 @@ __device__ __forceinline__ float row_lift(float top) {
     return top < 0x1p-60f ? 0x1p60f : top > 0x1p60f ? 0x1p-60f : 1.f;
 }
 
-// top / 127, correctly rounded: a quotient by the rounded 1 / 127 and one correction from its exact rest;
-// the plain division where the rest could be lost below the normal numbers
+// top / 127, correctly rounded: a quotient by the rounded 1 / 127 and one correction from its exact rest (Markstein,
+// IBM J. Res. Dev. 34, 1990); the plain division where the rest could be lost below the normal numbers
 __device__ __forceinline__ float row_scale(float top) {
     constexpr float r = 1.f / 127.f;
     const float q = top * r;
     return top > 0x1p-90f ? fmaf(fmaf(-q, 127.f, top), r, q) : top / 127.f;
 }
 
-// 1 / sqrt(a), a step of Newton's on the hardware's estimate (0 for an infinite a)
+// 1 / sqrt(a): rsqrtf and a step of Newton's iteration (0 for an infinite a)
 __device__ __forceinline__ float inv_sqrt(float a) {
     const float r = rsqrtf(a);
     return isinf(a) ? 0.f : fmaf(0.5f * r, fmaf(-a * r, r, 1.f), r);
 }
 
 // What a thread holds of a row: 8 * NCH elements, in 16-byte pieces of neighbours G pieces apart, or, where
-// rows are not aligned, single ones G apart.  `raw` keeps them as they lie in memory.  Pointers are those of the thread's first element, `left`
-// what the row has from there on.
+// rows are not aligned, single ones G apart.  `raw` keeps them as they lie in memory.  Pointers are those of the
+// thread's first element, `left` what the row has from there on.
 // FIT: kOdd rows are not aligned, kVec rows are, kFull rows are and fill their group (nothing lies past the end).
 enum Fit : int { kOdd, kVec, kFull };
 template <class T, int G, int NCH, Fit FIT>
