@@ -425,7 +425,7 @@ GCDR_API int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream);
  *
  * N1, N2 (post, pre): GCDR_NORM_LAYER (u - mean) / sqrt(var + eps) * g + b, GCDR_NORM_RMS
  * u / sqrt(mean(u^2) + eps) * g + b, or none (g and b are then not read); g and b are C floats,
- * 16-byte aligned ones are fastest, NULL: 1 and 0.  Everything is held
+ * 32-byte aligned ones are fastest, NULL: 1 and 0.  Everything is held
  * in fp32 (squares have to fit it) and rounded once, where it is stored: N2 sees v unrounded.
  *   x     residual stream, or NULL (none added);  f  the block's output, or NULL (v = x)
  *   gate  rows of C, row t / gate_rows for token t: gate_rows = rows one layer scale for all, tokens

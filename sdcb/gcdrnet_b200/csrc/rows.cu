@@ -121,7 +121,7 @@ extern "C" int gcdr_k_block_norm(const gcdr_block_norm_desc *d, void *stream) {
     a.qs = d->qs;
     const bool vec = C % 8 == 0 && aligned(d->x, d->ldx * size, 16) && aligned(d->f, d->ldf * size, 16) &&
                      aligned(d->gate, d->ldg * size, 16) && aligned(d->r, d->ldr * size, 16) &&
-                     aligned(d->y, d->ldy * size, 16) && aligned(d->q, d->ldq, 8) && aligned(g1, 16, 16) &&
-                     aligned(b1, 16, 16) && aligned(g2, 16, 16) && aligned(b2, 16, 16);
+                     aligned(d->y, d->ldy * size, 16) && aligned(d->q, d->ldq, 8) && aligned(g1, 0, 32) &&
+                     aligned(b1, 0, 32) && aligned(g2, 0, 32) && aligned(b2, 0, 32);
     return launch<false>(who, a, d->dtype, vec, static_cast<cudaStream_t>(stream));
 }

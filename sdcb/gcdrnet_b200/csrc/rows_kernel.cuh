@@ -185,19 +185,23 @@ struct RowPart {
             }
         }
     }
-    // the same from a table in shared memory that fills the whole group
-    static __device__ __forceinline__ void table4(uint32_t p, int k, float2 *v) {
-        if constexpr (VEC) {
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y) : "r"(p + 4u * at(4 * k)) : "memory");
-        } else {
+    // elements 8 k .. 8 k + 7 of 16-bit rows in one load of 32 bytes (two of 16 take twice the passes over the lines)
+    static __device__ __forceinline__ void param8(const float *p, int left, int k, float fill, float2 *v) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float t;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(t) : "r"(p + 4u * at(4 * k + e)) : "memory");
-                (e & 1 ? v[e / 2].y : v[e / 2].x) = t;
-            }
-        }
+        for (int i = 0; i < 4; i++) v[i] = make_float2(fill, fill);
+        if (in(8 * k, left))
+            asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[2].x), "=f"(v[2].y), "=f"(v[3].x), "=f"(v[3].y)
+                         : "l"(p + at(8 * k))
+                         : "memory");
     }
+    // the same from a table in shared memory that fills the whole group: four elements of each thread after the other
+    // threads' four, so that a load's 16-byte pieces are neighbours
+    static __device__ __forceinline__ void table4(uint32_t p, int k, float2 *v) {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y) : "r"(p + 16u * (G * k)) : "memory");
+    }
+    // the row's element at place i of the table
+    static __device__ __forceinline__ int table_at(int i) { return i / 4 % G * P + at(i / (4 * G) * 4 + i % 4); }
 };
 
 // The arithmetic of a row once its group holds it: 8 * NCH elements a thread, zeros past its end (and zeros they
@@ -208,11 +212,11 @@ struct RowMath {
     static constexpr bool VEC = FIT != kOdd;
     static constexpr int E = 8 * NCH;
     // 16-bit rows of a warp or less keep the gains and shifts in shared memory, 1 and 0 past the row and where there
-    // are none (57600 rows of 256 fp16, both norms, to int8: 28 us against 31 from L1, which the rows pass through; fp32
-    // rows, bound by their bytes, lose 3 % by it).
+    // are none (57600 rows of 256 fp16, both LayerNorm: 22 us against 27 from L1, where the rows pass through and the 32 bytes
+    // of a thread's eight elements take two passes; fp32 rows lose 3 % by it).
     static constexpr bool TABLE = G <= 32 && !QUANT && sizeof(T) == 2;
     static constexpr int W = G * E;         // floats of one of its four rows: g1, b1, g2, b2
-    uint32_t table = 0;                     // this thread's first element of g1
+    uint32_t table = 0;                     // this thread's first four elements of g1
     const RowArgs &a;
     Group<G> grp;
     const int first, left;                  // this thread's first element, and how many the row has from there
@@ -266,28 +270,40 @@ struct RowMath {
             }
         }
     }
+    // A gate's only row and the residual scale belong to the first norm's gain and shift (one product each less per
+    // element, and no loads of the gate).
+    __device__ __forceinline__ bool folded() const { return TABLE && a.post && a.gate && a.gate_rows >= a.rows; }
     // fills the table: every thread of the block, before the first norm
     __device__ __forceinline__ void fill(float *t) {
+        const T *gate = static_cast<const T *>(a.gate);
         for (int i = threadIdx.x; i < 4 * W; i += blockDim.x) {
-            const int row = i / W, c = i - row * W;
+            const int row = i / W, c = Part::table_at(i - row * W);
             const float *p = row == 0 ? a.g1 : row == 1 ? a.b1 : row == 2 ? a.g2 : a.b2;
-            t[i] = p && c < a.C ? p[c] : row & 1 ? 0.f : 1.f;
+            float v = p && c < a.C ? p[c] : row & 1 ? 0.f : 1.f;
+            if (folded() && row < 2 && c < a.C) v *= a.res_scale * to_f32(gate[c]);
+            t[i] = v;
         }
-        table = (uint32_t)__cvta_generic_to_shared(t) + 4u * first;
+        table = (uint32_t)__cvta_generic_to_shared(t) + 16u * (first / Part::P);
         __syncthreads();
     }
     template <bool GAIN, bool SHIFT>
     __device__ __forceinline__ void affine(float2 *v, float2 rstd, const float *g, const float *b) const {
+        constexpr int S = VEC && sizeof(T) == 2 ? 8 : 4;      // elements of a load
 #pragma unroll
-        for (int k = 0; k < E / 4; k++) {
-            float2 t[4];
-            if (GAIN) Part::param4(g, left, k, 1.f, t);
-            if (SHIFT) Part::param4(b, left, k, 0.f, t + 2);
+        for (int k = 0; k < E / S; k++) {
+            float2 tg[S / 2], tb[S / 2];
+            if constexpr (S == 8) {
+                if (GAIN) Part::param8(g, left, k, 1.f, tg);
+                if (SHIFT) Part::param8(b, left, k, 0.f, tb);
+            } else {
+                if (GAIN) Part::param4(g, left, k, 1.f, tg);
+                if (SHIFT) Part::param4(b, left, k, 0.f, tb);
+            }
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float2 &x = v[2 * k + i];
+            for (int i = 0; i < S / 2; i++) {
+                float2 &x = v[S / 2 * k + i];
                 x = __fmul2_rn(x, rstd);
-                x = GAIN && SHIFT ? __ffma2_rn(x, t[i], t[2 + i]) : GAIN ? __fmul2_rn(x, t[i]) : SHIFT ? __fadd2_rn(x, t[2 + i]) : x;
+                x = GAIN && SHIFT ? __ffma2_rn(x, tg[i], tb[i]) : GAIN ? __fmul2_rn(x, tg[i]) : SHIFT ? __fadd2_rn(x, tb[i]) : x;
             }
         }
     }
@@ -296,6 +312,14 @@ struct RowMath {
     __device__ __forceinline__ void join(float2 *v, const Part &gate, const Part &x) {
         if (a.post) norm(v, false);
         float2 t[E / 2];
+        if (folded()) {
+            if (a.x) {
+                x.get(t);
+#pragma unroll
+                for (int i = 0; i < E / 2; i++) v[i] = __fadd2_rn(v[i], t[i]);
+            }
+            return;
+        }
         if (a.gate) {
             gate.get(t);
 #pragma unroll
@@ -362,15 +386,13 @@ struct RowMath {
     }
 };
 
-// (two registers more than four blocks of 128 threads leave would cost the longest 16-bit norms a block: 16384 rows of
-// 4096 bf16, RMS, 88.8 us against 93.0)
 template <class T, int G, int NCH, Fit FIT, bool QUANT>
-__global__ void __launch_bounds__(G > 32 ? G : 256, G == 128 && NCH == 4 && FIT != kOdd ? 4 : 0) rows_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(G > 32 ? G : 256) rows_kernel(const __grid_constant__ RowArgs a) {
     constexpr int RPB = G > 32 ? 1 : 256 / G;   // rows per block
     using Math = RowMath<T, G, NCH, FIT, QUANT>;
     __shared__ float slots[G > 32 ? 2 * (G / 32) : 1];
     Math m(a, slots, threadIdx.x % G);
-    const bool has_x = QUANT || a.x, has_f = !QUANT && a.f, has_gate = has_f && a.gate;
+    const bool has_x = QUANT || a.x, has_f = !QUANT && a.f, has_gate = has_f && a.gate && !m.folded();
     const int64_t stride = (int64_t)gridDim.x * RPB;
     const int g = threadIdx.x / G;
     typename Math::Part x, f, gate;
@@ -439,10 +461,11 @@ cudaError_t launch_rows(const RowArgs &a, bool vec, cudaStream_t st) {
 }  // namespace
 
 // G and NCH by the row's length: 16 elements a thread, 24 where that leaves fewer threads idle (4099 rows of 1037 fp32
-// elements to int8: 64 x 24 4.7 us, 128 x 16 5.7).  The norms of long 16-bit rows, whose instructions and reductions bound
-// them, take 32 in half the threads (16384 rows of 4096 bf16, both RMS: 128 x 32 89 us, 256 x 16 106, 512 x 8 134; both
-// LayerNorm 123 against 143; 8192 rows of 2048, LayerNorm, 58 against 64); fp32 rows, bound by their bytes, do not (94 us
-// against 96).
+// elements to int8: 64 x 24 4.7 us, 128 x 16 5.7).  The norms of long 16-bit rows, whose reductions cost as much as their
+// bytes, take 32 in half the threads (both LayerNorm, bf16: 16384 rows of 4096 128 x 32 95 us, 256 x 16 108; 8192 of 8192
+// 256 x 32 107, 512 x 16 143; 16384 of 2048 64 x 32 48, 128 x 16 54); shorter rows, fp32 rows and the rounding alone do
+// not (1024 bf16 64 x 16 51 us, 32 x 32 50, RMS 46 and 49; 8192 to int8 512 x 16 40, 256 x 32 45).  Beyond 8192 the
+// registers of larger blocks decide (4096 rows of 16384 bf16, RMS: 512 x 32 97 us, 1024 x 16 147; to int8 46 and 41).
 template <class T, bool QUANT>
 cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st) {
     const auto fits = [&](int g, int nch) { return a.C <= 8 * g * nch; };
@@ -460,8 +483,10 @@ cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st) {
     if (fits(128, 3)) return launch_rows<T, 128, 3, QUANT>(a, vec, st);
     if (fits(128, 4)) return launch_rows<T, LONG ? 128 : 256, LONG ? 4 : 2, QUANT>(a, vec, st);
     if (fits(256, 3)) return launch_rows<T, 256, 3, QUANT>(a, vec, st);
-    if (fits(512, 2)) return launch_rows<T, 512, 2, QUANT>(a, vec, st);
-    if (fits(1024, 2)) return launch_rows<T, 1024, 2, QUANT>(a, vec, st);
+    if (fits(256, 4)) return launch_rows<T, LONG ? 256 : 512, LONG ? 4 : 2, QUANT>(a, vec, st);
+    if (!QUANT && fits(512, 3)) return launch_rows<T, 512, 3, QUANT>(a, vec, st);
+    if (fits(512, 4)) return launch_rows<T, QUANT ? 1024 : 512, QUANT ? 2 : 4, QUANT>(a, vec, st);
+    if (fits(1024, 3)) return launch_rows<T, 1024, 3, QUANT>(a, vec, st);
     return launch_rows<T, 1024, 4, QUANT>(a, vec, st);
 }
 
