@@ -554,6 +554,35 @@ def test_calls_back_to_back_on_reused_buffers():
             assert torch.equal(got, want)
 
 
+def test_calls_on_two_streams_at_once():
+    """Products of every form and norms on two streams side by side, many times over: the bytes of a call alone."""
+    import torch
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    jobs = []
+    for k, sizes in enumerate(([(4000, 2500, 3000), (16, 1000, 4000), (9001, 513, 1024)],
+                               [(2600, 4104, 4096), (3, 5000, 700), (1800, 512, 512), (12, 100, 4000)])):
+        for M, N, K in sizes:
+            x, xs, w, ws, b = _operands(M, N, K, M + N + k)
+            want = torch.empty(M, N, dtype=torch.float16, device="cuda:0")
+            assert i8_gemm(x, xs, w, ws, b, want) == 0
+            out = torch.zeros_like(want)
+            y, q, s = torch.zeros_like(want), torch.zeros(M, N, dtype=torch.int8, device="cuda:0"), torch.zeros(M, device="cuda:0")
+            ref = [torch.zeros_like(t) for t in (y, q, s)]
+            assert block_norm(x=want, pre=LAYER, y=ref[0], q=ref[1], qs=ref[2]) == 0
+            jobs.append((k, (x, xs, w, ws, b), want, out, (y, q, s), ref))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for k, ops, _, out, (y, q, s), _ in jobs:
+            st = streams[k].cuda_stream
+            assert i8_gemm(*ops, out, stream=st) == 0
+            assert block_norm(x=out, pre=LAYER, y=y, q=q, qs=s, stream=st) == 0
+    torch.cuda.synchronize()
+    for _, _, want, out, got, ref in jobs:
+        assert torch.equal(out, want)
+        for a, b in zip(got, ref):
+            assert torch.equal(a, b)
+
+
 def test_refusals_with_device_operands():
     """Host memory, overlapping operands: refused before anything is launched."""
     import torch
