@@ -62,44 +62,56 @@ struct Group {
     }
 };
 
-// v * 127 / top to nearest even, for a quotient that an estimate cannot tell from a border k + 1/2:
-// decided by the sign of 127 v - (k + 1/2) top, whose two products and their rests are exact in fp32
-// (31 and 32 bits).
-__device__ __noinline__ int round_at_border(float v, float top) {
-    const float k = floorf(v * 127.f / top), h = k + 0.5f;
-    const float p = __fmul_rn(127.f, v), pr = fmaf(127.f, v, -p);
-    const float m = __fmul_rn(h, top), mr = fmaf(h, top, -m);
-    const float d = (p - m) + (pr - mr);
-    return (int)(d > 0.f ? k + 1.f : d < 0.f ? k : 2.f * rintf(h * 0.5f));
-}
-
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Four values as int8, in order.  inv estimates 127 / top to 2^-22, so the quotient lies between the products with
-// lo = inv (1 - 2^-21) and hi = inv (1 + 2^-21); both are rounded by the addition of 1.5 * 2^23.  Where they differ a
-// border lies between, and the exact comparison decides.
+// Four values as int8, in order: v * 127 / top to nearest even, exactly.  inv estimates 127 / top to 2^-22, so the quotient
+// t lies between the products with lo = inv (1 - 2^-21) and hi = inv (1 + 2^-21); both are rounded by the addition of
+// 1.5 * 2^23.  Where they differ, a border k + 1/2 lies between.
+//   SHORT: v and top have 11 bits or fewer.  A quotient of theirs that is no border is at least t 2^-20 from one
+//     (254 v - (2 k + 1) top is a whole number of v's last places, each t / 254 of top's or more), further than
+//     lo and hi reach: t IS the border, and of k and k + 1 the even one is wanted.  Their sum, at twice the size,
+//     rounds to exactly that.  (Borders are common then: a bf16 row whose largest mantissa is 254 / 256 has half of
+//     its values on one.)
+//   else the sign of 127 v - (k + 1/2) top decides, whose two products and their rests are exact in fp32 (31 and 32
+//     bits).
+template <bool SHORT>
 __device__ __forceinline__ uint32_t round4(const float2 *v, float top, float lo, float hi) {
     constexpr float kMagic = 12582912.f;
-    uint32_t a[4], apart = 0;
+    uint32_t a[4];
+    if constexpr (SHORT) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const float2 p = __ffma2_rn(v[i], both(lo), both(kMagic)), q = __ffma2_rn(v[i], both(hi), both(kMagic));
-        a[2 * i] = __float_as_uint(p.x);
-        a[2 * i + 1] = __float_as_uint(p.y);
-        apart |= (a[2 * i] ^ __float_as_uint(q.x)) | (a[2 * i + 1] ^ __float_as_uint(q.y));
-    }
-    if (apart) {
+        for (int i = 0; i < 2; i++) {
+            const float2 s = __fadd2_rn(__ffma2_rn(v[i], both(lo), both(kMagic)), __ffma2_rn(v[i], both(hi), both(kMagic)));
+            a[2 * i] = __float_as_uint(s.x);
+            a[2 * i + 1] = __float_as_uint(s.y);
+        }
+    } else {
+        uint32_t c[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float x = i & 1 ? v[i / 2].y : v[i / 2].x;
-            if (a[i] != __float_as_uint(fmaf(x, hi, kMagic))) a[i] = (uint32_t)round_at_border(x, top);
+        for (int i = 0; i < 2; i++) {
+            const float2 p = __ffma2_rn(v[i], both(lo), both(kMagic)), q = __ffma2_rn(v[i], both(hi), both(kMagic));
+            a[2 * i] = __float_as_uint(p.x);
+            a[2 * i + 1] = __float_as_uint(p.y);
+            c[2 * i] = a[2 * i] ^ __float_as_uint(q.x);
+            c[2 * i + 1] = a[2 * i + 1] ^ __float_as_uint(q.y);
+        }
+        if (c[0] | c[1] | c[2] | c[3]) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x = i & 1 ? v[i / 2].y : v[i / 2].x;
+                const float k = floorf(x * lo), h = k + 0.5f;
+                const float p = __fmul_rn(127.f, x), m = __fmul_rn(h, top);
+                const float d = (p - m) + (fmaf(127.f, x, -p) - fmaf(h, top, -m));
+                const float q = d > 0.f ? k + 1.f : d < 0.f ? k : 2.f * rintf(h * 0.5f);
+                a[i] = c[i] ? __float_as_uint(q + kMagic) : a[i];
+            }
         }
     }
     return __byte_perm(__byte_perm(a[0], a[1], 0x0040), __byte_perm(a[2], a[3], 0x0040), 0x5410);
 }
 
 // Rows beyond these are scaled by a power of two first (exact), so that 127 / top and the
-// products of round_at_border stay normal numbers.
+// products of round4 stay normal numbers.
 __device__ __forceinline__ float row_lift(float top) {
     return top < 0x1p-60f ? 0x1p60f : top > 0x1p60f ? 0x1p-60f : 1.f;
 }
@@ -365,7 +377,7 @@ struct RowMath {
         uint32_t last = 0;
 #pragma unroll
         for (int i = 0; i < E / 4; i++) {
-            const uint32_t w = round4(v + 2 * i, top, lo, hi);
+            const uint32_t w = round4<QUANT && sizeof(T) == 2>(v + 2 * i, top, lo, hi);
             if constexpr (!VEC) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)

@@ -639,3 +639,26 @@ def test_i8_gemm_wait_runs_out_and_reports_timeout(case):
     assert L.gcdr_k_status(None) == 0
     want, bound = ref_product(x, xs, w, ws, None, False, torch.float32)
     assert worst(out, want, bound) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_quant_rows_every_quotient_of_16_bits(dtype):
+    """Every value of the type from the largest down to 2^-9 of it, against every mantissa of the largest: all borders
+    that 16-bit rows can meet, and their neighbours."""
+    import torch
+    dt = torch_dtype(dtype)
+    bits = 11 if dtype == "f16" else 8
+    mant = torch.arange(1 << (bits - 1), 1 << bits, device="cuda:0").double()      # every mantissa
+    for top_exp in (0, 4):
+        vals = torch.cat([mant * 2.0 ** (top_exp - e) for e in range(10)])
+        for part in mant.split(128):
+            top = part * 2.0 ** top_exp
+            x = torch.where(vals[None, :] <= top[:, None], vals[None, :], torch.zeros_like(vals)[None, :])
+            sign = torch.where(torch.arange(vals.numel(), device="cuda:0") % 2 == 0, 1.0, -1.0).double()
+            x = torch.cat([x * sign, top[:, None]], 1).to(dt)
+            x = (x.double() * 2.0 ** -6).to(dt)
+            q = torch.empty(x.shape, dtype=torch.int8, device="cuda:0")
+            s = torch.empty(x.shape[0], device="cuda:0")
+            assert quant_rows(x, q, s) == 0
+            wq, ws = ref_quant(x)
+            assert torch.equal(q, wq) and torch.equal(s, ws)
