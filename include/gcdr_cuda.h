@@ -377,7 +377,8 @@ GCDR_API int gcdr_k_conv_static(const gcdr_conv_desc *d, void *stream);
  * another operand, except that r and y of gcdr_k_block_norm may be x or f itself at the same pitch.  Zero
  * rows: GCDR_OK, nothing is launched.  A refused call prints the reason to stderr and launches
  * nothing: GCDR_ERR_ARG (null, unaligned, overlapping or foreign operands, unknown codes), GCDR_ERR_RANGE
- * (sizes and pitches).  The same call gives the same bytes, whatever runs beside it. */
+ * (sizes and pitches).  The same call gives the same bytes, whatever runs beside it, and a row's
+ * bytes do not depend on the call's other rows (at the same alignment). */
 #define GCDR_DTYPE_F16 0
 #define GCDR_DTYPE_BF16 1
 #define GCDR_DTYPE_F32 2

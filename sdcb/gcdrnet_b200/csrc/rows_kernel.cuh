@@ -282,18 +282,12 @@ struct RowMath {
             }
         }
     }
-    // A gate's only row and the residual scale belong to the first norm's gain and shift (one product each less per
-    // element, and no loads of the gate).
-    __device__ __forceinline__ bool folded() const { return TABLE && a.post && a.gate && a.gate_rows >= a.rows; }
     // fills the table: every thread of the block, before the first norm
     __device__ __forceinline__ void fill(float *t) {
-        const T *gate = static_cast<const T *>(a.gate);
         for (int i = threadIdx.x; i < 4 * W; i += blockDim.x) {
             const int row = i / W, c = Part::table_at(i - row * W);
             const float *p = row == 0 ? a.g1 : row == 1 ? a.b1 : row == 2 ? a.g2 : a.b2;
-            float v = p && c < a.C ? p[c] : row & 1 ? 0.f : 1.f;
-            if (folded() && row < 2 && c < a.C) v *= a.res_scale * to_f32(gate[c]);
-            t[i] = v;
+            t[i] = p && c < a.C ? p[c] : row & 1 ? 0.f : 1.f;
         }
         table = (uint32_t)__cvta_generic_to_shared(t) + 16u * (first / Part::P);
         __syncthreads();
@@ -324,14 +318,6 @@ struct RowMath {
     __device__ __forceinline__ void join(float2 *v, const Part &gate, const Part &x) {
         if (a.post) norm(v, false);
         float2 t[E / 2];
-        if (folded()) {
-            if (a.x) {
-                x.get(t);
-#pragma unroll
-                for (int i = 0; i < E / 2; i++) v[i] = __fadd2_rn(v[i], t[i]);
-            }
-            return;
-        }
         if (a.gate) {
             gate.get(t);
 #pragma unroll
@@ -404,7 +390,7 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) rows_kernel(const __grid_con
     using Math = RowMath<T, G, NCH, FIT, QUANT>;
     __shared__ float slots[G > 32 ? 2 * (G / 32) : 1];
     Math m(a, slots, threadIdx.x % G);
-    const bool has_x = QUANT || a.x, has_f = !QUANT && a.f, has_gate = has_f && a.gate && !m.folded();
+    const bool has_x = QUANT || a.x, has_f = !QUANT && a.f, has_gate = has_f && a.gate;
     const int64_t stride = (int64_t)gridDim.x * RPB;
     const int g = threadIdx.x / G;
     typename Math::Part x, f, gate;

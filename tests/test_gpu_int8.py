@@ -387,16 +387,23 @@ def test_block_norm_extremes():
 
 # ------------------------------------------------------------------ together, and how they are called
 
-def test_the_norm_does_not_depend_on_other_rows():
+@pytest.mark.parametrize("gate", ["all", 1, 50, None])
+@pytest.mark.parametrize("C", [96, 256, 1000, 4096])
+def test_the_norm_does_not_depend_on_other_rows(C, gate):
+    """A token's bytes are the same alone and in any batch, whatever the gate's rows are shared by."""
     import torch
-    t = _block(256, 300, "f16", LAYER, "all", LAYER)
+    t = _block(C, 300, "f16", LAYER, gate, LAYER)
     o = _norm_outputs(t)
     assert block_norm(**t, r=o["r"], y=o["y"], q=o["q"], qs=o["qs"]) == 0
-    one = {k: (v[17:18] if k in ("x", "f") else v) for k, v in t.items()}
-    p = _norm_outputs(one)
-    assert block_norm(**one, r=p["r"], y=p["y"], q=p["q"], qs=p["qs"]) == 0
-    for k in ("r", "y", "q", "qs"):
-        assert torch.equal(p[k], o[k][17:18])
+    for row in (17, 299):
+        one = {k: (v[row:row + 1] if k in ("x", "f") else v) for k, v in t.items()}
+        if gate is not None:
+            g = row // t["gate_rows"]
+            one.update(gate=t["gate"][g:g + 1], gate_rows=1)
+        p = _norm_outputs(one)
+        assert block_norm(**one, r=p["r"], y=p["y"], q=p["q"], qs=p["qs"]) == 0
+        for k in ("r", "y", "q", "qs"):
+            assert torch.equal(p[k], o[k][row:row + 1]), (k, row)
 
 
 def test_product_same_bytes_at_any_batch():
