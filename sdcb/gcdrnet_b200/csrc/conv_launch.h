@@ -51,9 +51,9 @@ int tc_pick_bk(int C);
 // 32/64/128), strides[i] = byte stride of dims[i + 1].
 bool tma_encode(CUtensorMap *m, const void *base, int rank, const uint64_t *dims, const uint64_t *strides,
                 const uint32_t *box, int swizzle_bytes, std::string &err);
-// int8 rows (the int8 token product): boxes of 128 bytes x box_rows rows.
-bool tma_encode_i8(CUtensorMap *m, const void *base, int64_t inner, int64_t rows, int64_t pitch, int box_rows,
-                   std::string &err);
+// Rows of 1-, 2- or 4-byte elements (the int8 token product): boxes of 64 or 128 bytes x box_rows rows.
+bool tma_encode_rows(CUtensorMap *m, const void *base, int size, int64_t inner, int64_t rows, int64_t pitch, int box_bytes,
+                     int box_rows, std::string &err);
 // The activation map of a conv (a.A): [nimg][a_rows][C] with the launch's image stride, a
 // box of box_inner channels x box_rows rows of one image.
 bool tma_encode_act(CUtensorMap *m, const ConvArgs &a, uint32_t box_inner, uint32_t box_rows, std::string &err);

@@ -401,19 +401,20 @@ bool tma_encode(CUtensorMap *m, const void *base, int rank, const uint64_t *dims
     return true;
 }
 
-// int8 rows of `inner` bytes `pitch` bytes apart, boxes of 128 bytes x box_rows rows (128-byte swizzle);
-// out-of-range bytes read as zero
-bool tma_encode_i8(CUtensorMap *m, const void *base, int64_t inner, int64_t rows, int64_t pitch, int box_rows,
-                   std::string &err) {
+// rows of `inner` elements (`size` bytes each: 1, 2, 4) `pitch` bytes apart, boxes of box_bytes (64 or 128, with that
+// swizzle) x box_rows rows; out-of-range elements read as zero and are not written
+bool tma_encode_rows(CUtensorMap *m, const void *base, int size, int64_t inner, int64_t rows, int64_t pitch, int box_bytes,
+                     int box_rows, std::string &err) {
     const auto encode = get_encoder(err);
     if (!encode) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, es[2] = {1, 1};
-    const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / size), (cuuint32_t)box_rows}, es[2] = {1, 1};
+    const CUresult r = encode(m, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32,
+                              2, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        err = "cuTensorMapEncodeTiled (int8) failed (" + std::to_string((int)r) + ")";
+        err = "cuTensorMapEncodeTiled (rows) failed (" + std::to_string((int)r) + ")";
         return false;
     }
     return true;
