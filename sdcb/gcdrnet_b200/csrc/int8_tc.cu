@@ -227,11 +227,15 @@ __device__ __forceinline__ void unit_tiles(const I8Plan &pl, int u, int &pt, int
     pt = g * pl.group + r - qt * n;
 }
 
-// CG: CTAs per unit.  EPI: epilogue warps.
-template <class T, bool NARROW, int CG, int EPI>
+// The result's map, a parameter of the kernels that store by it alone.
+template <bool STORE> struct OutMap { CUtensorMap map; };
+template <> struct OutMap<false> {};
+
+// CG: CTAs per unit.  EPI: epilogue warps.  STORE: results leave by tensor store.
+template <class T, bool NARROW, int CG, int EPI, bool STORE>
 __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
     i8_tc_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
-                 const __grid_constant__ CUtensorMap tmO, const __grid_constant__ I8Args a, const __grid_constant__ I8Plan pl) {
+                 const __grid_constant__ OutMap<STORE> out_map, const __grid_constant__ I8Args a, const __grid_constant__ I8Plan pl) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int bn = pl.bn;
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
     if (threadIdx.x == 32) {             // the tensor maps are on their way while the previous kernel ends
         prefetch_map(&tmP);
         prefetch_map(&tmQ);
-        if (!NARROW && pl.tma_out) prefetch_map(&tmO);
+        if constexpr (STORE) prefetch_map(&out_map.map);
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < pl.stages; s++) {
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                 const int c_end = a.N - n0 < bn ? (int)(a.N - n0) : bn;
                 const uint32_t scale = smem_u32(sc);
                 for (int c0 = part * CW; c0 < c_end; c0 += parts * CW) {
-                    if (pl.tma_out) {                         // the last piece has left the stage
+                    if (STORE) {                              // the last piece has left the stage
                         if (elect_one()) store_wait_read();
                         __syncwarp();
                     }
@@ -497,10 +501,10 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                             st_shared(put ^ (uint32_t)((h * (LW / E) + k) * 16), p);
                         }
                     }
-                    if (pl.tma_out) {
+                    if constexpr (STORE) {
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (mb < a.M && elect_one()) tma_store_2d(&tmO, stg, (int)(n0 + c0), (int)mb);
+                        if (mb < a.M && elect_one()) tma_store_2d(&out_map.map, stg, (int)(n0 + c0), (int)mb);
                         continue;
                     }
                     __syncwarp();
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                 aph ^= 1u;
             }
         }
-        if (!NARROW && pl.tma_out) {
+        if (STORE) {
             __syncwarp();
             if (elect_one()) store_wait_all();
         }
@@ -651,10 +655,12 @@ I8Plan plan_for(const I8Args &a, int sms) {
     return pl;
 }
 
-template <class T, bool NARROW, int CG, int EPI>
+template <class T, bool NARROW, int CG, int EPI, bool STORE>
 cudaError_t launch(const I8Args &a, const I8Plan &pl, const CUtensorMap &tp, const CUtensorMap &tq, const CUtensorMap &to, int sms,
                    cudaStream_t st) {
-    auto k = i8_tc_kernel<T, NARROW, CG, EPI>;
+    auto k = i8_tc_kernel<T, NARROW, CG, EPI, STORE>;
+    OutMap<STORE> out;
+    if constexpr (STORE) out.map = to;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap);
     if (e != cudaSuccess) return e;
     const int64_t units = (int64_t)pl.tiles_p * pl.tiles_q;
@@ -679,15 +685,22 @@ cudaError_t launch(const I8Args &a, const I8Plan &pl, const CUtensorMap &tp, con
     }
     cfg.attrs = at;
     cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, k, tp, tq, to, a, pl);
+    return cudaLaunchKernelEx(&cfg, k, tp, tq, out, a, pl);
+}
+
+template <class T, bool STORE>
+cudaError_t launch_wide(const I8Args &a, const I8Plan &pl, const CUtensorMap &tp, const CUtensorMap &tq, const CUtensorMap &to,
+                        int sms, cudaStream_t st) {
+    if (pl.pair) return launch<T, false, 2, 8, STORE>(a, pl, tp, tq, to, sms, st);
+    return pl.epi == 16 ? launch<T, false, 1, 16, STORE>(a, pl, tp, tq, to, sms, st)
+                        : launch<T, false, 1, 8, STORE>(a, pl, tp, tq, to, sms, st);
 }
 
 template <class T>
 cudaError_t launch_form(const I8Args &a, const I8Plan &pl, const CUtensorMap &tp, const CUtensorMap &tq, const CUtensorMap &to,
                         int sms, cudaStream_t st) {
-    if (pl.narrow) return launch<T, true, 1, 8>(a, pl, tp, tq, to, sms, st);
-    if (pl.pair) return launch<T, false, 2, 8>(a, pl, tp, tq, to, sms, st);
-    return pl.epi == 16 ? launch<T, false, 1, 16>(a, pl, tp, tq, to, sms, st) : launch<T, false, 1, 8>(a, pl, tp, tq, to, sms, st);
+    if (pl.narrow) return launch<T, true, 1, 8, false>(a, pl, tp, tq, to, sms, st);
+    return pl.tma_out ? launch_wide<T, true>(a, pl, tp, tq, to, sms, st) : launch_wide<T, false>(a, pl, tp, tq, to, sms, st);
 }
 
 }  // namespace
@@ -700,7 +713,7 @@ int i8_tc_launch(const I8Args &a, cudaStream_t st, std::string &err) {
     I8Plan pl = plan_for(a, sms);
     const int64_t units = (int64_t)pl.tiles_p * pl.tiles_q;
     if (units > (1 << 30)) { err = "too many tiles"; return -1; }
-    CUtensorMap tx, tw, to = {};
+    CUtensorMap tx, tw, to;
     const int q_box = pl.bn / (pl.pair ? 2 : 1);
     if (!tma_encode_rows(&tx, a.x, 1, a.K, a.M, a.ldx, kBlockK, pl.narrow ? q_box : 128, err) ||
         !tma_encode_rows(&tw, a.w, 1, a.K, a.N, a.ldw, kBlockK, pl.narrow ? 128 : q_box, err))
