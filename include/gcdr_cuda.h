@@ -393,8 +393,8 @@ GCDR_API int gcdr_k_conv_static(const gcdr_conv_desc *d, void *stream);
 GCDR_API int gcdr_k_quant_rows(const void *x, int dtype, int64_t rows, int C, int64_t ldx, int8_t *q,
                                int64_t ldq, float *scale, void *stream);
 
-/* out[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], then relu (a NaN stays NaN), rounded to
- * `dtype`.  The integer sum is exact: K 1..131071 (int32 sums of products up to 2^14).
+/* out[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], then relu (a NaN stays NaN, a zero has no
+ * sign), rounded to `dtype`.  The integer sum is exact: K 1..131071 (int32 sums of products up to 2^14).
  *   x    int8 [M][K], pitch ldx, xs M scales;   w  int8 [N][K], pitch ldw, ws N scales
  *        x and w 16-byte aligned, ldx and ldw multiples of 16 (K and N are free); rows on
  *        128-byte lines (ldx, ldw multiples of 128) read up to twice as fast

@@ -174,13 +174,7 @@ __device__ __forceinline__ void free_tmem(uint32_t base, uint32_t cols) {
         tmem_dealloc(base, cols);
 }
 
-// max(v, 0), a NaN stays
-__device__ __forceinline__ float relu(float v) {
-    float m;
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(m) : "f"(v));
-    return m;
-}
-
+// relu_f32 of two packed results
 __device__ __forceinline__ uint32_t relu2(uint32_t v, __half) {
     const __half2 h = __hmax2_nan(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(0)));
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -485,10 +479,10 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                                 const float2 v0 = __ffma2_rn(__fmul2_rn(make_float2((float)q[0], (float)q[1]), rs2), make_float2(w.x, w.y), make_float2(c.x, c.y));
                                 const float2 v1 = __ffma2_rn(__fmul2_rn(make_float2((float)q[2], (float)q[3]), rs2), make_float2(w.z, w.w), make_float2(c.z, c.w));
                                 if constexpr (sizeof(T) == 4) {
-                                    p[0] = __float_as_uint(a.relu ? relu(v0.x) : v0.x);
-                                    p[1] = __float_as_uint(a.relu ? relu(v0.y) : v0.y);
-                                    p[2] = __float_as_uint(a.relu ? relu(v1.x) : v1.x);
-                                    p[3] = __float_as_uint(a.relu ? relu(v1.y) : v1.y);
+                                    p[0] = __float_as_uint(a.relu ? relu_f32(v0.x) : v0.x);
+                                    p[1] = __float_as_uint(a.relu ? relu_f32(v0.y) : v0.y);
+                                    p[2] = __float_as_uint(a.relu ? relu_f32(v1.x) : v1.x);
+                                    p[3] = __float_as_uint(a.relu ? relu_f32(v1.y) : v1.y);
                                 } else {
                                     p[2 * i] = pack2(v0.x, v0.y, T());
                                     p[2 * i + 1] = pack2(v1.x, v1.y, T());
@@ -550,6 +544,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
     if (NARROW && split > 1) {
         // join: a CTA that gave up says so to all, the sums of the others are then not used
         if (threadIdx.x < split && *abort_flag) st_cluster(map_to(smem_u32(&sh->peer_abort), threadIdx.x), 1);
+        __syncwarp();
         cluster_sync();
         if (first < units && !*const_cast<volatile int *>(&sh->peer_abort)) {
             int pt, qt;

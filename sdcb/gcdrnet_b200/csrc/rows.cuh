@@ -58,11 +58,18 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// max(v, 0): a NaN stays, a zero has no sign
+__device__ __forceinline__ float relu_f32(float v) {
+    float m;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(m) : "f"(v));
+    return m;
+}
+
 // One result of the int8 product: a rounding of the sum's (up to 31) bits to fp32 and two of the scaling.  The sum
 // takes one scale, then the other: the product of the two alone could leave the normal numbers.
 __device__ __forceinline__ float i8_result(int acc, float xs, float ws, float bias, bool relu) {
     const float v = fmaf((float)acc * xs, ws, bias);
-    return relu && v < 0.f ? 0.f : v;   // (a NaN stays)
+    return relu ? relu_f32(v) : v;
 }
 
 }  // namespace gcdr

@@ -418,6 +418,30 @@ def test_product_same_bytes_at_any_batch():
         assert torch.equal(out, full[:m]), m
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("relu", [False, True])
+def test_product_same_bytes_of_zeros_and_nan_at_any_batch(dtype, relu):
+    """Results that round to a negative zero, and NaN, have the same bytes in every form too; after relu a zero has no
+    sign."""
+    import torch
+    n = 200
+    x, xs, w, ws, _ = _operands(40000, n, 96, 8)
+    xs[0::3] = 1e-30
+    ws[0::2] = 1e-30                        # (their products underflow, half of them from below)
+    xs[1] = float("nan")
+    whole = torch.int32 if dtype == "f32" else torch.int16
+    full = torch.empty(40000, n, device="cuda:0", dtype=torch_dtype(dtype))
+    assert i8_gemm(x, xs, w, ws, None, full, relu) == 0
+    negative = (full == 0) & torch.signbit(full)
+    assert negative.any().item() != relu
+    assert torch.isnan(full[1]).all()
+    for m in (2, 4, 8, 40, 300, 2000):
+        out = torch.empty(m, n, device="cuda:0", dtype=full.dtype)
+        assert i8_gemm(x[:m], xs[:m], w, ws, None, out, relu) == 0
+        differ = (out.view(whole) != full[:m].view(whole)).sum().item()
+        assert differ == 0, (m, differ)
+
+
 @pytest.mark.parametrize("net,name", [("gc", "block1"), ("dr", "block2")])
 def test_shifted_mlp_block_in_8_bits(net, name):
     """One shifted-MLP block on int8 products, as a deployment chains the entries: norm with int8 rows -> fc1 ->
