@@ -587,12 +587,17 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
     }
 }
 
+uintptr_t result_place(const I8Args &a) {   // what the starts of the result's rows are multiples of
+    return reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * dtype_bytes(a.dtype));
+}
+
 // Picks form and tile by an estimate in SM cycles, fitted to measured sweeps (B200, K 256 to 8192, 16 to 57600
 // tokens, 160 to 8192 channels; within 15 % of the best form there):
 //   a k-block step     what its loads and MMAs take together (a pair's for twice the rows; the second figures where
 //                      rows do not start on a line: each 128 bytes are then two requests); 16 epilogue warps leave a
 //                      ring stage less
-//   a unit's results   at 12 bytes per cycle with 8 epilogue warps (64-byte stores), 16 with 16 of them
+//   a unit's results   at 12 bytes per cycle with 8 epilogue warps (64-byte stores), 16 with 16 of them; rows that start
+//                      at multiples of 8 bytes only 8 and 12 (10 of 256), at any element 6 and 9 (8)
 //   a round            700 between units; the last one's results and the start are not hidden (nor, of two units, the
 //                      second half of the warps)
 //   a split of K       the join's words through distributed shared memory; clusters of eight fit the GPU 12 times
@@ -616,13 +621,16 @@ I8Plan plan_for(const I8Args &a, int sms) {
     };
     const bool cut = (a.ldx | a.ldw) % 128 != 0;   // a box's 128 bytes lie in two lines each
     const int64_t m128 = div(a.M, 128);
+    const uintptr_t odd = result_place(a);
+    const int e8 = odd % 16 == 0 ? 12 : odd % 8 == 0 ? 8 : 6;
     for (int bn = 64; bn <= 256; bn *= 2) {
         const int64_t tq = div(a.N, bn), units = m128 * tq, rounds = div(units, sms);
-        const int64_t work = kb * (cut ? (bn == 256 ? 1300 : bn == 128 ? 950 : 670) : bn == 256 ? 740 : bn == 128 ? 430 : 300), bytes = 128ll * (a.N < bn ? a.N : bn) * size;
+        const int64_t work = kb * (cut ? (bn == 256 ? 1300 : bn == 128 ? 950 : 670) : bn == 256 ? 740 : bn == 128 ? 430 : 300), bytes = 128 * div(a.N, tq) * size;
+        const int e16 = odd % 16 == 0 ? 16 : odd % 8 == 0 ? (bn == 256 ? 10 : 12) : bn == 256 ? 8 : 9;
         const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 700) + (w > e ? e : w) + (r == 2 ? e : 0); };
-        offer(cost(rounds, work, bytes / 12) + 1500, 0, 0, 8, bn, 1);
-        if (rounds > 2) offer(cost(rounds, work * 11 / 10, bytes / 16) + 2000, 0, 0, 16, bn, 1);
-        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * (cut ? 1000 : 650), bytes / 12) + 5500, 0, 1, 8, bn, 1);
+        offer(cost(rounds, work, bytes / e8) + 1500, 0, 0, 8, bn, 1);
+        if (rounds > 2) offer(cost(rounds, work * 11 / 10, bytes / e16) + 2000, 0, 0, 16, bn, 1);
+        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * (cut ? 1000 : 650), bytes / e8) + 5500, 0, 1, 8, bn, 1);
         if (a.N <= bn) break;
     }
     const int64_t n128 = div(a.N, 128);
@@ -717,7 +725,7 @@ int i8_tc_launch(const I8Args &a, cudaStream_t st, std::string &err) {
     // Several units a CTA: their results leave by tensor store (57600 x 512 x 512 fp16 21.8 us, 23.0 by the warps; a
     // single unit gains nothing by it, and its caller waits for the map).  A tensor store writes whole 16-byte pieces:
     // a row that ended inside one would spill into the space behind it.
-    const uintptr_t odd = reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * size) | (uintptr_t)((int64_t)a.N * size);
+    const uintptr_t odd = result_place(a) | (uintptr_t)((int64_t)a.N * size);
     pl.tma_out = !pl.narrow && units > (pl.pair ? sms / 2 : sms) && odd % 16 == 0 && a.ldo < (int64_t)1 << 36;
     if (pl.tma_out && !tma_encode_rows(&to, a.out, size, a.N, a.M, a.ldo * size, row_bytes(pl.epi), 32, err)) return -1;
     const CUtensorMap &tp = pl.narrow ? tw : tx, &tq = pl.narrow ? tx : tw;
