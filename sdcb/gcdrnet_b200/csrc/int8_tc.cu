@@ -25,6 +25,7 @@
 #include <cuda_runtime.h>
 
 #include <string>
+#include <type_traits>
 
 #include "conv_launch.h"
 #include "int8.h"
@@ -192,23 +193,41 @@ __device__ __forceinline__ void st_shared(uint32_t p, const uint32_t *v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 
-// A store stage's rows of RB bytes to rows at any element, V at a time
-template <class V, int RB, class T>
-__device__ __forceinline__ void store_rows(const uint8_t *from, T *to, int64_t ldo, int rows, int cols, int lane) {
-    constexpr int E = sizeof(V) / sizeof(T), LR = RB / (int)sizeof(V), CL = LR < 32 ? LR : 32, RO = 32 / CL, PC = RB / 16;
-#pragma unroll 4
-    for (int r = lane / CL; r < rows; r += RO) {
-        const int x = PC == 8 ? r & 7 : (r >> 1) & 3;
+__device__ __forceinline__ uint16_t ld_shared(uint32_t p, uint16_t) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_shared(uint32_t p, uint32_t) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 ld_shared(uint32_t p, uint2) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
+    return v;
+}
+
+// A store stage's rows of RB bytes to rows at any element, V at a time; what is left of `cols` behind the last whole V
+// goes element by element (U: one as its bits)
+template <class V, class U, int RB>
+__device__ __forceinline__ void store_rows(uint32_t from, U *to, int64_t ldo, int rows, int cols, int lane) {
+    constexpr int E = sizeof(V) / sizeof(U), LR = RB / (int)sizeof(V), CL = LR < 32 ? LR : 32, RO = 32 / CL, PC = RB / 16;
+    const auto at = [&](int r, int byte) { return from + (uint32_t)(r * RB + (byte ^ (PC == 8 ? r & 7 : (r >> 1) & 3) << 4)); };
+    const int c = lane % CL, r0 = lane / CL, whole = cols / E;
+    U *q = to + r0 * ldo + c * E;
+    const int64_t step = RO * ldo;
+#pragma unroll 8
+    for (int i = 0; i < CL; i++, q += step) {
 #pragma unroll
-        for (int i = 0; i < LR / CL; i++) {
-            const int c = lane % CL + i * CL, byte = c * (int)sizeof(V);
-            const uint8_t *p = from + r * RB + (((byte >> 4) ^ x) << 4) + (byte & 15);
-            T *q = to + r * ldo + c * E;
-            if ((c + 1) * E <= cols) *reinterpret_cast<V *>(q) = *reinterpret_cast<const V *>(p);
-            else
-                for (int k = 0; c * E + k < cols; k++) q[k] = reinterpret_cast<const T *>(p)[k];
+        for (int k = 0; k < LR; k += CL) {
+            const V v = ld_shared(at(r0 + i * RO, (c + k) * (int)sizeof(V)), V());
+            if (r0 + i * RO < rows && c + k < whole) *reinterpret_cast<V *>(q + k * E) = v;
         }
     }
+    if (E > 1 && lane < rows)
+        for (int k = whole * E; k < cols; k++) to[lane * ldo + k] = ld_shared(at(lane, k * (int)sizeof(U)), U());
 }
 
 // Unit u -> its P and Q tiles: `group` P tiles per Q tile, then the next Q tile.
@@ -513,12 +532,12 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                     } else {
                         // results at odd places, or a row's last piece cut short
                         const unsigned odd = (unsigned)(reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * (int64_t)sizeof(T))) & 15u;
-                        const uint8_t *from = extra + e * 32 * RB;
-                        T *to = static_cast<T *>(a.out) + mb * a.ldo + n0 + c0;
+                        using U = typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type;
+                        U *to = static_cast<U *>(a.out) + mb * a.ldo + n0 + c0;
                         const int rows = a.M - mb < 32 ? (int)(a.M - mb) : 32, cols = c_end - c0;
-                        if (odd % 8 == 0) store_rows<uint2, RB>(from, to, a.ldo, rows, cols, lane);
-                        else if (sizeof(T) == 4 || odd % 4 == 0) store_rows<uint32_t, RB>(from, to, a.ldo, rows, cols, lane);
-                        else store_rows<T, RB>(from, to, a.ldo, rows, cols, lane);
+                        if (odd % 8 == 0) store_rows<uint2, U, RB>(stg, to, a.ldo, rows, cols, lane);
+                        else if (sizeof(T) == 4 || odd % 4 == 0) store_rows<uint32_t, U, RB>(stg, to, a.ldo, rows, cols, lane);
+                        else store_rows<U, U, RB>(stg, to, a.ldo, rows, cols, lane);
                     }
                     __syncwarp();
                 }
@@ -597,7 +616,7 @@ uintptr_t result_place(const I8Args &a) {   // what the starts of the result's r
 //                      rows do not start on a line: each 128 bytes are then two requests); 16 epilogue warps leave a
 //                      ring stage less
 //   a unit's results   at 12 bytes per cycle with 8 epilogue warps (64-byte stores), 16 with 16 of them; rows that start
-//                      at multiples of 8 bytes only 8 and 12 (10 of 256), at any element 6 and 9 (8)
+//                      at multiples of 8 bytes only 10 (a pair 8) and 13, at any element 8 (6) and 11
 //   a round            700 between units; the last one's results and the start are not hidden (nor, of two units, the
 //                      second half of the warps)
 //   a split of K       the join's words through distributed shared memory; clusters of eight fit the GPU 12 times
@@ -622,15 +641,15 @@ I8Plan plan_for(const I8Args &a, int sms) {
     const bool cut = (a.ldx | a.ldw) % 128 != 0;   // a box's 128 bytes lie in two lines each
     const int64_t m128 = div(a.M, 128);
     const uintptr_t odd = result_place(a);
-    const int e8 = odd % 16 == 0 ? 12 : odd % 8 == 0 ? 8 : 6;
+    const int e8 = odd % 16 == 0 ? 12 : odd % 8 == 0 ? 10 : 8, pair8 = odd % 16 == 0 ? 12 : odd % 8 == 0 ? 8 : 6;
     for (int bn = 64; bn <= 256; bn *= 2) {
         const int64_t tq = div(a.N, bn), units = m128 * tq, rounds = div(units, sms);
         const int64_t work = kb * (cut ? (bn == 256 ? 1300 : bn == 128 ? 950 : 670) : bn == 256 ? 740 : bn == 128 ? 430 : 300), bytes = 128 * div(a.N, tq) * size;
-        const int e16 = odd % 16 == 0 ? 16 : odd % 8 == 0 ? (bn == 256 ? 10 : 12) : bn == 256 ? 8 : 9;
+        const int e16 = odd % 16 == 0 ? 16 : odd % 8 == 0 ? (bn == 256 ? 11 : 13) : bn == 256 ? 10 : 11;
         const auto cost = [](int64_t r, int64_t w, int64_t e) { return r * ((w > e ? w : e) + 700) + (w > e ? e : w) + (r == 2 ? e : 0); };
         offer(cost(rounds, work, bytes / e8) + 1500, 0, 0, 8, bn, 1);
         if (rounds > 2) offer(cost(rounds, work * 11 / 10, bytes / e16) + 2000, 0, 0, 16, bn, 1);
-        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * (cut ? 1000 : 650), bytes / e8) + 5500, 0, 1, 8, bn, 1);
+        if (bn == 256 && a.M > 128) offer(cost(div(div(a.M, 256) * tq, sms / 2), kb * (cut ? 1000 : 650), bytes / pair8) + 5500, 0, 1, 8, bn, 1);
         if (a.N <= bn) break;
     }
     const int64_t n128 = div(a.N, 128);
