@@ -9,16 +9,15 @@ namespace gcdr {
 namespace {
 
 template <bool QUANT>
-int launch(const char *who, const RowArgs &a, int dtype, bool vec, cudaStream_t st) {
-    const cudaError_t e = dtype == GCDR_DTYPE_F16    ? rows_launch<__half, QUANT>(a, vec, st)
-                          : dtype == GCDR_DTYPE_BF16 ? rows_launch<__nv_bfloat16, QUANT>(a, vec, st)
-                                                     : rows_launch<float, QUANT>(a, vec, st);
+int launch(const char *who, const RowArgs &a, int dtype, int piece, cudaStream_t st) {
+    const cudaError_t e = dtype == GCDR_DTYPE_F16    ? rows_launch<__half, QUANT>(a, piece, st)
+                          : dtype == GCDR_DTYPE_BF16 ? rows_launch<__nv_bfloat16, QUANT>(a, piece, st)
+                                                     : rows_launch<float, QUANT>(a, piece, st);
     if (e == cudaSuccess) return GCDR_OK;
     cudaGetLastError();
     return refuse(who, GCDR_ERR_DEVICE, cudaGetErrorString(e));
 }
 
-// 16-byte vectors of an activation row, 8-byte ones of an int8 row
 bool aligned(const void *p, int64_t ld_bytes, int n) {
     return !p || (reinterpret_cast<uintptr_t>(p) % n == 0 && ld_bytes % n == 0);
 }
@@ -50,8 +49,9 @@ extern "C" int gcdr_k_quant_rows(const void *x, int dtype, int64_t rows, int C, 
     a.q = q;
     a.ldq = ldq;
     a.qs = scale;
-    const bool vec = C % 8 == 0 && aligned(x, ldx * size, 16) && aligned(q, ldq, 8);
-    return launch<true>(who, a, dtype, vec, static_cast<cudaStream_t>(stream));
+    // n elements at a time: pieces of an activation's row and of an int8 row
+    const auto whole = [&](int n, int bytes) { return C % n == 0 && aligned(x, ldx * size, bytes) && aligned(q, ldq, n); };
+    return launch<true>(who, a, dtype, whole(8, 16) ? 16 : whole(2, 2 * size) ? 2 : 0, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int gcdr_k_block_norm(const gcdr_block_norm_desc *d, void *stream) {
@@ -119,9 +119,11 @@ extern "C" int gcdr_k_block_norm(const gcdr_block_norm_desc *d, void *stream) {
     a.q = d->q;
     a.ldq = d->ldq;
     a.qs = d->qs;
-    const bool vec = C % 8 == 0 && aligned(d->x, d->ldx * size, 16) && aligned(d->f, d->ldf * size, 16) &&
-                     aligned(d->gate, d->ldg * size, 16) && aligned(d->r, d->ldr * size, 16) &&
-                     aligned(d->y, d->ldy * size, 16) && aligned(d->q, d->ldq, 8) && aligned(g1, 0, 32) &&
-                     aligned(b1, 0, 32) && aligned(g2, 0, 32) && aligned(b2, 0, 32);
-    return launch<false>(who, a, d->dtype, vec, static_cast<cudaStream_t>(stream));
+    // n elements at a time: pieces of the activations' rows, of an int8 row and of the gains and shifts
+    const auto whole = [&](int n, int bytes) {
+        return C % n == 0 && aligned(d->x, d->ldx * size, bytes) && aligned(d->f, d->ldf * size, bytes) &&
+               aligned(d->gate, d->ldg * size, bytes) && aligned(d->r, d->ldr * size, bytes) && aligned(d->y, d->ldy * size, bytes) &&
+               aligned(d->q, d->ldq, n) && aligned(g1, 0, 4 * n) && aligned(b1, 0, 4 * n) && aligned(g2, 0, 4 * n) && aligned(b2, 0, 4 * n);
+    };
+    return launch<false>(who, a, d->dtype, whole(8, 16) ? 16 : whole(2, 2 * size) ? 2 : 0, static_cast<cudaStream_t>(stream));
 }

@@ -2,6 +2,6 @@
 #include "rows_kernel.cuh"
 
 namespace gcdr {
-template cudaError_t rows_launch<float, true>(const RowArgs &, bool, cudaStream_t);
-template cudaError_t rows_launch<float, false>(const RowArgs &, bool, cudaStream_t);
+template cudaError_t rows_launch<float, true>(const RowArgs &, int, cudaStream_t);
+template cudaError_t rows_launch<float, false>(const RowArgs &, int, cudaStream_t);
 }  // namespace gcdr

@@ -131,16 +131,19 @@ __device__ __forceinline__ float inv_sqrt(float a) {
 }
 
 // What a thread holds of a row: 8 * NCH elements, in 16-byte pieces of neighbours G pieces apart, or, where
-// rows are not aligned, single ones G apart.  `raw` keeps them as they lie in memory.  Pointers are those of the
+// rows are not aligned, pairs or single ones G apart.  `raw` keeps them as they lie in memory.  Pointers are those of the
 // thread's first element, `left` what the row has from there on.
-// FIT: kOdd rows are not aligned, kVec rows are, kFull rows are and fill their group (nothing lies past the end).
-enum Fit : int { kOdd, kVec, kFull };
+// FIT: kOdd rows start anywhere, kPair rows are whole pairs of elements (8192 x 2046 fp16, both LayerNorm and a gate: 33 us
+// against 44 by single elements; to int8 9.9 and 13.1; fp32 norm 55 and 57), kVec rows whole 16-byte pieces, kFull rows
+// too and fill their group (nothing lies past the end).
+enum Fit : int { kOdd, kPair, kVec, kFull };
 template <class T, int G, int NCH, Fit FIT>
 struct RowPart {
-    static constexpr bool VEC = FIT != kOdd;
+    static constexpr bool VEC = FIT >= kVec;
     static constexpr int E = 8 * NCH;
-    static constexpr int P = VEC ? 16 / (int)sizeof(T) : 1;        // elements of a piece
-    using Raw = typename std::conditional<VEC, uint4, T>::type;
+    static constexpr int P = VEC ? 16 / (int)sizeof(T) : FIT == kPair ? 2 : 1;        // elements of a piece
+    using Pair = typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type;
+    using Raw = typename std::conditional<VEC, uint4, typename std::conditional<FIT == kPair, Pair, T>::type>::type;
     Raw raw[E / P];
     static __device__ __forceinline__ constexpr int at(int j) { return j / P * G * P + j % P; }
     static __device__ __forceinline__ bool in(int j, int left) { return FIT == kFull || at(j) < left; }
@@ -148,15 +151,19 @@ struct RowPart {
 #pragma unroll
         for (int i = 0; i < E / P; i++) {
             if (in(i * P, left)) raw[i] = *reinterpret_cast<const Raw *>(p + at(i * P));
-            else if constexpr (VEC) raw[i] = make_uint4(0, 0, 0, 0);
+            else if constexpr (P > 1) raw[i] = Raw();
             else raw[i] = from_f32<T>(0.f);
         }
     }
     __device__ __forceinline__ void get(float2 *v) const {
 #pragma unroll
         for (int i = 0; i < E / P; i++) {
-            if constexpr (!VEC) {
+            if constexpr (P == 1) {
                 (i & 1 ? v[i / 2].y : v[i / 2].x) = to_f32(raw[i]);
+            } else if constexpr (!VEC && sizeof(T) == 4) {
+                v[i] = make_float2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y));
+            } else if constexpr (!VEC) {
+                unpack2(raw[i], &v[i].x, T());
             } else if constexpr (sizeof(T) == 4) {
                 v[2 * i] = make_float2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y));
                 v[2 * i + 1] = make_float2(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w));
@@ -172,8 +179,12 @@ struct RowPart {
 #pragma unroll
         for (int i = 0; i < E / P; i++) {
             if (!in(i * P, left)) continue;
-            if constexpr (!VEC) {
+            if constexpr (P == 1) {
                 p[at(i)] = from_f32<T>(i & 1 ? v[i / 2].y : v[i / 2].x);
+            } else if constexpr (!VEC && sizeof(T) == 4) {
+                *reinterpret_cast<float2 *>(p + at(2 * i)) = v[i];
+            } else if constexpr (!VEC) {
+                *reinterpret_cast<uint32_t *>(p + at(2 * i)) = pack2(v[i].x, v[i].y, T());
             } else if constexpr (sizeof(T) == 4) {
                 *reinterpret_cast<float4 *>(p + at(4 * i)) = make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
             } else {
@@ -189,6 +200,10 @@ struct RowPart {
             const float4 t = in(4 * k, left) ? *reinterpret_cast<const float4 *>(p + at(4 * k)) : make_float4(fill, fill, fill, fill);
             v[0] = make_float2(t.x, t.y);
             v[1] = make_float2(t.z, t.w);
+        } else if constexpr (P == 2) {
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                v[e] = in(4 * k + 2 * e, left) ? *reinterpret_cast<const float2 *>(p + at(4 * k + 2 * e)) : both(fill);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -221,7 +236,7 @@ struct RowPart {
 template <class T, int G, int NCH, Fit FIT, bool QUANT>
 struct RowMath {
     using Part = RowPart<T, G, NCH, FIT>;
-    static constexpr bool VEC = FIT != kOdd;
+    static constexpr bool VEC = FIT >= kVec;
     static constexpr int E = 8 * NCH;
     // 16-bit rows of a warp or less keep the gains and shifts in shared memory, 1 and 0 past the row and where there
     // are none (57600 rows of 256 fp16, both LayerNorm: 22 us against 27 from L1, where the rows pass through and the 32 bytes
@@ -364,7 +379,11 @@ struct RowMath {
 #pragma unroll
         for (int i = 0; i < E / 4; i++) {
             const uint32_t w = round4<QUANT && sizeof(T) == 2>(v + 2 * i, top, lo, hi);
-            if constexpr (!VEC) {
+            if constexpr (FIT == kPair) {
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (Part::in(4 * i + 2 * e, n)) *reinterpret_cast<uint16_t *>(p + Part::at(4 * i + 2 * e)) = (uint16_t)(w >> (16 * e));
+            } else if constexpr (!VEC) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (Part::in(4 * i + e, n)) p[Part::at(4 * i + e)] = (int8_t)(w >> (8 * e));
@@ -451,9 +470,9 @@ cudaError_t launch_rows(const RowArgs &a, cudaStream_t st) {
 }
 
 template <class T, int G, int NCH, bool QUANT>
-cudaError_t launch_rows(const RowArgs &a, bool vec, cudaStream_t st) {
-    return !vec ? launch_rows<T, G, NCH, kOdd, QUANT>(a, st) : a.C == 8 * G * NCH ? launch_rows<T, G, NCH, kFull, QUANT>(a, st)
-                                                                                 : launch_rows<T, G, NCH, kVec, QUANT>(a, st);
+cudaError_t launch_rows(const RowArgs &a, int piece, cudaStream_t st) {
+    if (piece < 16) return piece ? launch_rows<T, G, NCH, kPair, QUANT>(a, st) : launch_rows<T, G, NCH, kOdd, QUANT>(a, st);
+    return a.C == 8 * G * NCH ? launch_rows<T, G, NCH, kFull, QUANT>(a, st) : launch_rows<T, G, NCH, kVec, QUANT>(a, st);
 }
 
 }  // namespace
@@ -465,27 +484,27 @@ cudaError_t launch_rows(const RowArgs &a, bool vec, cudaStream_t st) {
 // not (1024 bf16 64 x 16 51 us, 32 x 32 50, RMS 46 and 49; 8192 to int8 512 x 16 40, 256 x 32 45).  Beyond 8192 the
 // registers of larger blocks decide (4096 rows of 16384 bf16, RMS: 512 x 32 97 us, 1024 x 16 147; to int8 46 and 41).
 template <class T, bool QUANT>
-cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st) {
+cudaError_t rows_launch(const RowArgs &a, int piece, cudaStream_t st) {
     const auto fits = [&](int g, int nch) { return a.C <= 8 * g * nch; };
     constexpr bool LONG = !QUANT && sizeof(T) == 2;
-    if (fits(8, 1)) return launch_rows<T, 8, 1, QUANT>(a, vec, st);
-    if (fits(8, 2)) return launch_rows<T, 8, 2, QUANT>(a, vec, st);
-    if (fits(8, 3)) return launch_rows<T, 8, 3, QUANT>(a, vec, st);
-    if (fits(16, 2)) return launch_rows<T, 16, 2, QUANT>(a, vec, st);
-    if (fits(16, 3)) return launch_rows<T, 16, 3, QUANT>(a, vec, st);
-    if (fits(32, 2)) return launch_rows<T, 32, 2, QUANT>(a, vec, st);
-    if (fits(32, 3)) return launch_rows<T, 32, 3, QUANT>(a, vec, st);
-    if (fits(64, 2)) return launch_rows<T, 64, 2, QUANT>(a, vec, st);
-    if (fits(64, 3)) return launch_rows<T, 64, 3, QUANT>(a, vec, st);
-    if (fits(64, 4)) return launch_rows<T, LONG ? 64 : 128, LONG ? 4 : 2, QUANT>(a, vec, st);
-    if (fits(128, 3)) return launch_rows<T, 128, 3, QUANT>(a, vec, st);
-    if (fits(128, 4)) return launch_rows<T, LONG ? 128 : 256, LONG ? 4 : 2, QUANT>(a, vec, st);
-    if (fits(256, 3)) return launch_rows<T, 256, 3, QUANT>(a, vec, st);
-    if (fits(256, 4)) return launch_rows<T, LONG ? 256 : 512, LONG ? 4 : 2, QUANT>(a, vec, st);
-    if (!QUANT && fits(512, 3)) return launch_rows<T, 512, 3, QUANT>(a, vec, st);
-    if (fits(512, 4)) return launch_rows<T, QUANT ? 1024 : 512, QUANT ? 2 : 4, QUANT>(a, vec, st);
-    if (fits(1024, 3)) return launch_rows<T, 1024, 3, QUANT>(a, vec, st);
-    return launch_rows<T, 1024, 4, QUANT>(a, vec, st);
+    if (fits(8, 1)) return launch_rows<T, 8, 1, QUANT>(a, piece, st);
+    if (fits(8, 2)) return launch_rows<T, 8, 2, QUANT>(a, piece, st);
+    if (fits(8, 3)) return launch_rows<T, 8, 3, QUANT>(a, piece, st);
+    if (fits(16, 2)) return launch_rows<T, 16, 2, QUANT>(a, piece, st);
+    if (fits(16, 3)) return launch_rows<T, 16, 3, QUANT>(a, piece, st);
+    if (fits(32, 2)) return launch_rows<T, 32, 2, QUANT>(a, piece, st);
+    if (fits(32, 3)) return launch_rows<T, 32, 3, QUANT>(a, piece, st);
+    if (fits(64, 2)) return launch_rows<T, 64, 2, QUANT>(a, piece, st);
+    if (fits(64, 3)) return launch_rows<T, 64, 3, QUANT>(a, piece, st);
+    if (fits(64, 4)) return launch_rows<T, LONG ? 64 : 128, LONG ? 4 : 2, QUANT>(a, piece, st);
+    if (fits(128, 3)) return launch_rows<T, 128, 3, QUANT>(a, piece, st);
+    if (fits(128, 4)) return launch_rows<T, LONG ? 128 : 256, LONG ? 4 : 2, QUANT>(a, piece, st);
+    if (fits(256, 3)) return launch_rows<T, 256, 3, QUANT>(a, piece, st);
+    if (fits(256, 4)) return launch_rows<T, LONG ? 256 : 512, LONG ? 4 : 2, QUANT>(a, piece, st);
+    if (!QUANT && fits(512, 3)) return launch_rows<T, 512, 3, QUANT>(a, piece, st);
+    if (fits(512, 4)) return launch_rows<T, QUANT ? 1024 : 512, QUANT ? 2 : 4, QUANT>(a, piece, st);
+    if (fits(1024, 3)) return launch_rows<T, 1024, 3, QUANT>(a, piece, st);
+    return launch_rows<T, 1024, 4, QUANT>(a, piece, st);
 }
 
 }  // namespace gcdr

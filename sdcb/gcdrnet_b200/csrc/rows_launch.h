@@ -36,8 +36,8 @@ struct RowArgs {
     float *qs;
 };
 
-// vec: every row of every operand is made of whole aligned 16-byte pieces
+// Aligned pieces that every row of every operand is made of: 16 bytes, 2 elements, or 0: single elements
 template <class T, bool QUANT>
-cudaError_t rows_launch(const RowArgs &a, bool vec, cudaStream_t st);
+cudaError_t rows_launch(const RowArgs &a, int piece, cudaStream_t st);
 
 }  // namespace gcdr

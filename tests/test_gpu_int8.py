@@ -320,6 +320,41 @@ def test_block_norm_pitches(case, pad):
     _check_norm(t, _norm_outputs(t, pad))
 
 
+# rows of whole pairs of elements that are no whole vectors: by their length, by their pitch, at every size of a group
+PAIRS = [(2, 9, 0), (10, 70, 0), (64, 33, 2), (130, 40, 4), (166, 21, 2), (250, 131, 0), (322, 9, 6), (510, 17, 0), (766, 5, 2),
+         (1026, 6, 0), (1534, 4, 10), (2046, 5, 0), (4092, 3, 0), (4622, 3, 2), (8190, 2, 0), (12286, 2, 0), (32766, 2, 2)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C,rows,pad", PAIRS)
+def test_rows_of_whole_pairs(C, rows, pad, dtype):
+    import torch
+    t = _block(C, rows, dtype, LAYER, 2, LAYER, seed=9, pad=pad)
+    _check_norm(t, _norm_outputs(t, pad))
+    q, qb = strided(rows, C, C + 2 * pad, torch.int8, 99)
+    s = torch.full((rows,), -1.0, device="cuda:0")
+    assert quant_rows(t["x"], q, s) == 0
+    wq, ws = ref_quant(t["x"])
+    assert torch.equal(q, wq) and torch.equal(s, ws) and untouched(q, qb, 99)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_at_every_start(dtype):
+    """Operands that start at each place of a 16-byte piece in turn, gains and shifts at each float of 32 bytes."""
+    import torch
+    C = 130
+    for start in range(1, 9):
+        t = _block(C, 6, dtype, LAYER, 1, LAYER, seed=start)
+        for name in ("x", "f", "gate", "g1", "b1", "g2", "b2"):
+            for only in (name, None) if start < 3 else (None,):
+                u = dict(t)
+                for k in ("x", "f", "gate", "g1", "b1", "g2", "b2"):
+                    if only in (None, k):
+                        b = torch.empty(t[k].numel() + start, device="cuda:0", dtype=t[k].dtype)[start:]
+                        u[k] = b.view(t[k].shape).copy_(t[k])
+                _check_norm(u, _norm_outputs(u))
+
+
 @pytest.mark.parametrize("C", [64, 100, 512, 3000])
 def test_block_norm_parts(C):
     """Each operand and each output left out in turn; norms without gain or shift."""
