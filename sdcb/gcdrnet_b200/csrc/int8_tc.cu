@@ -534,7 +534,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
                         const unsigned odd = (unsigned)(reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * (int64_t)sizeof(T))) & 15u;
                         using U = typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type;
                         U *to = static_cast<U *>(a.out) + mb * a.ldo + n0 + c0;
-                        const int rows = a.M - mb < 32 ? (int)(a.M - mb) : 32, cols = c_end - c0;
+                        const int rows = a.M - mb < 32 ? (int)(a.M - mb) : 32, cols = c_end - c0 < CW ? c_end - c0 : CW;
                         if (odd % 8 == 0) store_rows<uint2, U, RB>(stg, to, a.ldo, rows, cols, lane);
                         else if (sizeof(T) == 4 || odd % 4 == 0) store_rows<uint32_t, U, RB>(stg, to, a.ldo, rows, cols, lane);
                         else store_rows<U, U, RB>(stg, to, a.ldo, rows, cols, lane);

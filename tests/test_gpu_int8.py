@@ -183,6 +183,23 @@ def test_i8_gemm_result_alignments(M, N, dtype):
         assert untouched(out, buf, 9.0), (off, more)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,pad", [(2904, 183, 3), (2904, 183, 1), (300, 183, 5), (2904, 189, 3), (20000, 503, 1), (20000, 502, 2),
+                                     (9000, 1001, 3), (9000, 2047, 1)])
+def test_i8_gemm_rows_that_end_inside_a_piece(M, N, pad, dtype):
+    """Rows at multiples of 4 or 8 bytes whose last elements fill no such piece, after many that do (in several runs: the
+    pieces are stored side by side)."""
+    import torch
+    dt = torch_dtype(dtype)
+    x, xs, w, ws, b = _operands(M, N, 40, N)
+    want, bound = ref_product(x, xs, w, ws, b, False, dt)
+    for _ in range(3):
+        out, buf = strided(M, N, N + pad, dt, 9.0)
+        assert i8_gemm(x, xs, w, ws, b, out) == 0
+        assert worst(out, want, bound) <= 1.0
+        assert untouched(out, buf, 9.0)
+
+
 @pytest.mark.parametrize("M,N", [(1, 40), (24, 70), (200, 130)])
 def test_i8_gemm_largest_sums(M, N):
     """-128 x -128 over the longest rows the sum allows: 2^31 - 2^14, and its mirror."""
