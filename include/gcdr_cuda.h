@@ -418,6 +418,22 @@ typedef struct {
     int timeout_probe;
 } gcdr_i8_gemm_desc;
 GCDR_API int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream);
+/* The kernel that gcdr_k_i8_gemm takes for `d` on a device of `sms` SMs, for profiles and tests: the host
+ * decides by sizes, pitches, type and the alignment of `out` alone.  Touches no device and reads no operand.
+ *   form    0: M = 0, nothing is launched;  DOT (up to four tokens)  a warp for `tile` channels
+ *           WIDE    units of 128 tokens x `tile` channels;  PAIR  256 tokens x `tile` channels over two CTAs
+ *           NARROW  units of 128 channels x `tile` tokens, K split over `split` CTAs
+ *   units, epilogue_warps, accumulators (in TMEM), stages (of the operand ring); tensor_store: results leave by
+ *   tensor store */
+#define GCDR_I8_DOT 1
+#define GCDR_I8_NARROW 2
+#define GCDR_I8_WIDE 3
+#define GCDR_I8_PAIR 4
+typedef struct {
+    int form, tile, split, epilogue_warps, accumulators, tensor_store, stages;
+    int64_t units;
+} gcdr_i8_form;
+GCDR_API int gcdr_k_i8_gemm_form(const gcdr_i8_gemm_desc *d, int sms, gcdr_i8_form *form);
 
 /* The norms around a block, with its gate and residual scale, in one pass:
  *

@@ -22,7 +22,7 @@ import os
 import threading
 
 __all__ = ["GcdrBackend", "GcdrPixelFormat", "GcdrEnhancer", "CudaWorker", "ConvDesc", "I8GemmDesc",
-           "BlockNormDesc", "check", "lib", "library_path",
+           "I8GemmForm", "BlockNormDesc", "check", "lib", "library_path",
            "register_host", "unregister_host", "GcdrError", "ArgumentError", "ArgumentOutOfRangeError", "NotSupportedError",
            "DeviceLostError", "DeviceTimeoutError", "ModelError", "OutOfMemoryError",
            "bytes_per_pixel"]
@@ -116,6 +116,12 @@ class I8GemmDesc(ctypes.Structure):
                 ("timeout_probe", ctypes.c_int)]
 
 
+class I8GemmForm(ctypes.Structure):
+    """gcdr_i8_form of include/gcdr_cuda.h (gcdr_k_i8_gemm_form: the kernel a product takes)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("form", "tile", "split", "epilogue_warps", "accumulators", "tensor_store",
+                                            "stages")] + [("units", ctypes.c_int64)]
+
+
 class BlockNormDesc(ctypes.Structure):
     """gcdr_block_norm_desc of include/gcdr_cuda.h (gcdr_k_block_norm: the norms, gate and residual of a block)."""
     _fields_ = [("rows", ctypes.c_int64), ("C", ctypes.c_int), ("dtype", ctypes.c_int), ("x", ctypes.c_void_p),
@@ -198,6 +204,7 @@ def lib():
         L.gcdr_k_ln_finalize.argtypes = [vp, i, i, i, i, vp, vp, vp, vp, f, vp, vp, f, vp, vp, vp, vp]
         L.gcdr_k_quant_rows.argtypes = [vp, i, i64, i, i64, vp, i64, vp, vp]
         L.gcdr_k_i8_gemm.argtypes = [vp, vp]
+        L.gcdr_k_i8_gemm_form.argtypes = [vp, i, vp]
         L.gcdr_k_block_norm.argtypes = [vp, vp]
         _lib = L
         return L

@@ -162,10 +162,12 @@ cudaError_t launch_dot(const I8Args &a, cudaStream_t st) {
     return launch_pdl(i8_dot_kernel<T, MT, R, U>, dim3((unsigned)(((int64_t)a.N + 4 * R - 1) / (4 * R))), dim3(128), 0, st, a);
 }
 
+// Channels of a warp (few of them: a warp each, so that they spread over the GPU)
+int dot_channels(const I8Args &a) { return a.N < 4096 ? 1 : 2; }
+
 template <class T>
 cudaError_t launch_dot(const I8Args &a, cudaStream_t st) {
-    // few channels: a warp each, so that they spread over the GPU
-    const bool few = a.N < 4096;
+    const bool few = dot_channels(a) == 1;
     if (a.M == 1) return few ? launch_dot<T, 1, 1, 4>(a, st) : launch_dot<T, 1, 2, 4>(a, st);
     if (a.M == 2) return few ? launch_dot<T, 2, 1, 4>(a, st) : launch_dot<T, 2, 2, 4>(a, st);
     return few ? launch_dot<T, 4, 1, 4>(a, st) : launch_dot<T, 4, 2, 4>(a, st);
@@ -177,14 +179,51 @@ cudaError_t launch_dot(const I8Args &a, cudaStream_t st) {
 
 using namespace gcdr;
 
-extern "C" int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream) {
-    const char *who = "gcdr_k_i8_gemm";
+namespace {
+
+// What a descriptor may hold, as far as the host can tell without the device
+int check_desc(const char *who, const gcdr_i8_gemm_desc *d) {
     if (!d) return refuse(who, GCDR_ERR_ARG, "null descriptor");
-    const int size = dtype_bytes(d->dtype);
-    if (!size) return refuse(who, GCDR_ERR_ARG, "unknown dtype");
+    if (!dtype_bytes(d->dtype)) return refuse(who, GCDR_ERR_ARG, "unknown dtype");
     if (d->M < 0 || d->M > 0x7FFFFFFF || d->N < 1 || d->K < 1 || d->K > 131071)
         return refuse(who, GCDR_ERR_RANGE, "M must be 0..2^31-1, N >= 1 and K 1..131071");
     if (d->wait_cycles < 0) return refuse(who, GCDR_ERR_RANGE, "wait_cycles must be >= 0");
+    return GCDR_OK;
+}
+
+I8Args args_of(const gcdr_i8_gemm_desc *d) {
+    return {d->M, d->N, d->K, d->x, d->ldx, d->xs, d->w, d->ldw, d->ws, d->bias, d->relu, d->dtype, d->out, d->ldo,
+            d->wait_cycles, d->timeout_probe != 0};
+}
+
+bool by_dots(const I8Args &a) { return a.M <= kDotTokens && !a.timeout_probe; }
+
+}  // namespace
+
+extern "C" int gcdr_k_i8_gemm_form(const gcdr_i8_gemm_desc *d, int sms, gcdr_i8_form *form) {
+    const char *who = "gcdr_k_i8_gemm_form";
+    const int rc = check_desc(who, d);
+    if (rc) return rc;
+    if (!form) return refuse(who, GCDR_ERR_ARG, "null form");
+    if (sms < 2 || sms > 4096) return refuse(who, GCDR_ERR_RANGE, "sms must be 2..4096");
+    *form = {};
+    const I8Args a = args_of(d);
+    if (!a.M) return GCDR_OK;
+    if (!by_dots(a)) {
+        i8_tc_form(a, sms, *form);
+        return GCDR_OK;
+    }
+    form->form = GCDR_I8_DOT;
+    form->tile = dot_channels(a);
+    form->units = ((int64_t)a.N + form->tile - 1) / form->tile;
+    return GCDR_OK;
+}
+
+extern "C" int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream) {
+    const char *who = "gcdr_k_i8_gemm";
+    const int bad = check_desc(who, d);
+    if (bad) return bad;
+    const int size = dtype_bytes(d->dtype);
     if (d->M == 0) return GCDR_OK;
     if (!d->x || !d->xs || !d->w || !d->ws || !d->out) return refuse(who, GCDR_ERR_ARG, "null operand");
     if (((uintptr_t)d->x | (uintptr_t)d->w) % 16 || d->ldx % 16 || d->ldw % 16)
@@ -197,10 +236,9 @@ extern "C" int gcdr_k_i8_gemm(const gcdr_i8_gemm_desc *d, void *stream) {
                                         {"out", d->out, d->M, d->N, d->ldo, size, kOut}});
     if (rc) return rc;
     if (d->ldx >= (int64_t)1 << 40 || d->ldw >= (int64_t)1 << 40) return refuse(who, GCDR_ERR_RANGE, "a pitch of 2^40 or more");
-    const I8Args a = {d->M, d->N, d->K, d->x, d->ldx, d->xs, d->w, d->ldw, d->ws, d->bias, d->relu, d->dtype, d->out, d->ldo,
-                      d->wait_cycles, d->timeout_probe != 0};
+    const I8Args a = args_of(d);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.M > kDotTokens || a.timeout_probe) {
+    if (!by_dots(a)) {
         try {
             std::string err;
             return i8_tc_launch(a, st, err) ? refuse(who, GCDR_ERR_DEVICE, err.c_str()) : GCDR_OK;

@@ -6,6 +6,8 @@
 
 #include <string>
 
+#include "gcdr_cuda.h"
+
 namespace gcdr {
 
 constexpr int GCDR_ERR_FLAG_OTHER = 1 << 30;   // the status itself could not be read
@@ -31,5 +33,8 @@ struct I8Args {
 
 // The tensor-core kernel (int8_tc.cu); 0, or -1 and why not.
 int i8_tc_launch(const I8Args &a, cudaStream_t st, std::string &err);
+
+// The form that launch takes on a device of `sms` SMs (host only).
+void i8_tc_form(const I8Args &a, int sms, gcdr_i8_form &f);
 
 }  // namespace gcdr

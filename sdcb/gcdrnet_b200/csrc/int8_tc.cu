@@ -674,6 +674,11 @@ I8Plan plan_for(const I8Args &a, int sms) {
     const int room = kSmemCap - 1024 - pl.extra_bytes - (int)sizeof(I8Shared);
     pl.stages = room / (kPBytes + pl.bn / (pl.pair ? 2 : 1) * kBlockK);
     if (pl.stages > kRingStages) pl.stages = kRingStages;
+    // Several units a CTA: their results leave by tensor store (57600 x 512 x 512 fp16 21.8 us, 23.0 by the warps; a
+    // single unit gains nothing by it, and its caller waits for the map).  A tensor store writes whole 16-byte pieces:
+    // a row that ended inside one would spill into the space behind it.
+    pl.tma_out = !pl.narrow && (int64_t)pl.tiles_p * pl.tiles_q > (pl.pair ? sms / 2 : sms) &&
+                 (odd | (uintptr_t)((int64_t)a.N * size)) % 16 == 0 && a.ldo < (int64_t)1 << 36;
     return pl;
 }
 
@@ -741,11 +746,6 @@ int i8_tc_launch(const I8Args &a, cudaStream_t st, std::string &err) {
         !tma_encode_rows(&tw, a.w, 1, a.K, a.N, a.ldw, kBlockK, pl.narrow ? 128 : q_box, err))
         return -1;
     const int size = dtype_bytes(a.dtype);
-    // Several units a CTA: their results leave by tensor store (57600 x 512 x 512 fp16 21.8 us, 23.0 by the warps; a
-    // single unit gains nothing by it, and its caller waits for the map).  A tensor store writes whole 16-byte pieces:
-    // a row that ended inside one would spill into the space behind it.
-    const uintptr_t odd = result_place(a) | (uintptr_t)((int64_t)a.N * size);
-    pl.tma_out = !pl.narrow && units > (pl.pair ? sms / 2 : sms) && odd % 16 == 0 && a.ldo < (int64_t)1 << 36;
     if (pl.tma_out && !tma_encode_rows(&to, a.out, size, a.N, a.M, a.ldo * size, row_bytes(pl.epi), 32, err)) return -1;
     const CUtensorMap &tp = pl.narrow ? tw : tx, &tq = pl.narrow ? tx : tw;
     e = a.dtype == GCDR_DTYPE_F16    ? launch_form<__half>(a, pl, tp, tq, to, sms, st)
@@ -757,6 +757,18 @@ int i8_tc_launch(const I8Args &a, cudaStream_t st, std::string &err) {
         return -1;
     }
     return 0;
+}
+
+void i8_tc_form(const I8Args &a, int sms, gcdr_i8_form &f) {
+    const I8Plan pl = plan_for(a, sms);
+    f.form = pl.narrow ? GCDR_I8_NARROW : pl.pair ? GCDR_I8_PAIR : GCDR_I8_WIDE;
+    f.tile = pl.bn;
+    f.split = pl.split;
+    f.epilogue_warps = pl.epi;
+    f.accumulators = pl.bufs;
+    f.tensor_store = pl.tma_out;
+    f.stages = pl.stages;
+    f.units = (int64_t)pl.tiles_p * pl.tiles_q;
 }
 
 int i8_status_word() {
