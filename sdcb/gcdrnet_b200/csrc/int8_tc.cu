@@ -145,6 +145,15 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
         mma_commit(bar);
 }
 
+// The same on this CTA's barrier alone: the other CTA of a pair does not wait for it, and could be gone when it arrives.
+template <int CG>
+__device__ __forceinline__ void commit_own(uint64_t *bar) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else
+        mma_commit(bar);
+}
+
 // A box of one of the pair's CTAs, counted by the leader's barrier (`bar`: its shared::cluster address)
 __device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
     asm volatile(
@@ -358,7 +367,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
             }
             sh->consumed = consumed;
             if (*abort_flag) {   // every MMA issued is done (bounded) before TMEM is freed
-                commit<CG>(&sh->mdone);
+                commit_own<CG>(&sh->mdone);
                 const long long t0 = clock64();
                 while (!mbar_try(&sh->mdone, 0) && clock64() - t0 < kWaitCycles) {}
             }

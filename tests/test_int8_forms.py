@@ -164,3 +164,41 @@ def test_results_of_every_form(case):
         want, bound = ref_product(x, xs, w, ws, bias, relu, dt)
         assert worst(out, want, bound) <= 1.0
         assert untouched(out, buf, 123.0)
+
+
+# a case of each kernel's way out when a wait ends (the largest tiles and clusters, one and several units a CTA)
+GIVE_UP = [(NARROW, 128, 1, 8, 2, 0), (NARROW, 16, 2, 8, 2, 0), (NARROW, 64, 4, 8, 2, 0), (NARROW, 16, 8, 8, 2, 0),
+           (WIDE, 64, 1, 8, 1, 0), (WIDE, 128, 1, 8, 2, 0), (WIDE, 128, 1, 8, 2, 1), (WIDE, 64, 1, 16, 4, 0), (WIDE, 128, 1, 16, 4, 1),
+           (WIDE, 256, 1, 16, 2, 1), (PAIR, 256, 1, 8, 1, 0), (PAIR, 256, 1, 8, 2, 0), (PAIR, 256, 1, 8, 2, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("form", GIVE_UP, ids=lambda f: _id((f, "")))
+def test_every_kernel_gives_up_and_reports_timeout(form, dtype):
+    """The test hook issues no copies and no MMAs, so every role's first wait runs out (0.2 ms): nothing is written, the
+    status says so once, the kernel's TMEM is free again and the next call of the same kernel is right."""
+    import time
+
+    import torch
+    from int8_util import i8_gemm, ref_product, strided, torch_dtype, worst
+    from test_gpu_int8 import _operands
+    L = lib()
+    M, N, K, pad = FORMS[form][dtype == "f32"]
+    dt = torch_dtype(dtype)
+    x, xs, w, ws, b = _operands(M, N, K, M + N + K)
+    out, buf = strided(M, N, N + pad, dt, float("nan"))
+    want, bound = ref_product(x, xs, w, ws, b, False, dt)
+    torch.cuda.synchronize()
+    assert L.gcdr_k_status(None) == OK
+    assert _taken(x, w, out, timeout_probe=1) == form
+    for _ in range(3):
+        t0 = time.perf_counter()
+        assert i8_gemm(x, xs, w, ws, b, out, wait_cycles=400_000, timeout_probe=1) == 0
+        assert L.gcdr_k_status(None) == 5
+        assert time.perf_counter() - t0 < 5.0
+        assert torch.isnan(buf).all().item(), "the probe wrote outputs"
+        assert L.gcdr_k_status(None) == OK
+    assert i8_gemm(x, xs, w, ws, b, out) == 0
+    assert L.gcdr_k_status(None) == OK
+    assert worst(out, want, bound) <= 1.0
