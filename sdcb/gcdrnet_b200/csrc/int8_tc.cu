@@ -69,6 +69,7 @@ struct I8Shared {
     uint32_t tmem_base;
     int abort_flag, peer_abort;
     int issued, consumed;
+    int peer_count;          // of a pair's other CTA, if it gave up: stages issued (told to the leader) or consumed
 };
 
 // One lane of the (converged) warp
@@ -164,6 +165,10 @@ __device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map,
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Takes bytes that no copy will bring off a phase's count
+__device__ __forceinline__ void mbar_complete_tx(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void fence_acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
         }
         mbar_init(&sh->mdone, 1);
         sh->abort_flag = sh->peer_abort = 0;
-        sh->issued = sh->consumed = 0;
+        sh->issued = sh->consumed = sh->peer_count = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
@@ -593,21 +598,45 @@ __global__ void __launch_bounds__((kFirstEpi + EPI) * 32, 1)
             }
         }
     }
+    const auto done = [&](uint64_t *bars, int use) {    // the use-th phase of a ring's barriers (counted from 0)
+        const long long t0 = clock64();
+        while (!mbar_try(&bars[use % pl.stages], (uint32_t)((use / pl.stages) & 1)) && clock64() - t0 < kWaitCycles) {}
+    };
     if (threadIdx.x == 0) {
-        // copies issued but never consumed (only after an abort; the leader's barrier counts those of both CTAs of a
-        // pair), then the arrivals of the last commits
-        for (int g = sh->consumed; (CG == 1 || rank == 0) && g < sh->issued; g++) {
-            const long long t0 = clock64();
-            while (!mbar_try(&sh->full[g % pl.stages], (uint32_t)((g / pl.stages) & 1)) && clock64() - t0 < kWaitCycles) {}
-        }
-        const int done = CG == 2 && rank ? sh->issued : sh->consumed;
-        if (done > 0) {
-            const long long t0 = clock64();
-            while (!mbar_try(&sh->empty[(done - 1) % pl.stages], (uint32_t)(((done - 1) / pl.stages) & 1)) && clock64() - t0 < kWaitCycles) {}
+        if (CG == 2 && *abort_flag) {    // the other CTA hears of it, and how far this one came
+            st_cluster(map_to(smem_u32(&sh->peer_count), rank ^ 1), rank ? sh->issued : sh->consumed);
+            st_cluster(map_to(smem_u32(&sh->peer_abort), rank ^ 1), 1);
+        } else {
+            // copies issued but never consumed (only after an abort), then the arrivals of the last commits (a CTA of a
+            // pair that did not give up has seen all its units through: what it has issued is consumed)
+            for (int g = sh->consumed; CG == 1 && g < sh->issued; g++) done(sh->full, g);
+            const int last = CG == 2 ? sh->issued : sh->consumed;
+            if (last > 0) done(sh->empty, last - 1);
         }
     }
     __syncthreads();
-    if (CG == 2) cluster_sync();         // neither CTA's memory goes while the other's MMAs or arrivals may use it
+    if (CG == 2) {
+        cluster_sync();                  // neither CTA's memory goes while the other's MMAs or arrivals may use it
+        const bool peer = *const_cast<volatile int *>(&sh->peer_abort);
+        if (peer || *abort_flag) {
+            if (threadIdx.x == 0) {
+                const int count = *const_cast<volatile int *>(&sh->peer_count);
+                const int consumed = rank == 0 ? sh->consumed : peer ? count : sh->issued;
+                const int other = rank == 0 && peer ? count : consumed;      // (issued by the other CTA)
+                // Copies never consumed.  The leader's barriers count those of both CTAs; a stage that one of the two
+                // has issued alone is waited for by that one's bytes.
+                for (int g = consumed; rank == 0 && (g < sh->issued || g < other); g++) {
+                    uint64_t *bar = &sh->full[g % pl.stages];
+                    if (g >= other) mbar_complete_tx(bar, (uint32_t)stage_bytes);
+                    if (g >= sh->issued) mbar_expect_tx(bar, (uint32_t)stage_bytes);
+                    done(sh->full, g);
+                }
+                if (consumed > 0) done(sh->empty, consumed - 1);
+            }
+            __syncwarp();
+            cluster_sync();
+        }
+    }
     if (warp == 2) {
         __syncwarp();
         tc_fence_after();

@@ -202,3 +202,37 @@ def test_every_kernel_gives_up_and_reports_timeout(form, dtype):
     assert i8_gemm(x, xs, w, ws, b, out) == 0
     assert L.gcdr_k_status(None) == OK
     assert worst(out, want, bound) <= 1.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", GIVE_UP, ids=lambda f: _id((f, "")))
+def test_a_wait_that_ends_in_the_middle(form):
+    """A limit so short that real work runs into it: copies and MMAs are on their way when the kernel gives up.  It drains
+    them and returns; what it has stored is right, what it has not stands as it was, and the status tells the two apart."""
+    import time
+
+    import torch
+    from int8_util import i8_gemm, ref_product, strided, torch_dtype, worst
+    from test_gpu_int8 import _operands
+    L = lib()
+    M, N, K, pad = FORMS[form][0]
+    dt = torch_dtype("f16")
+    x, xs, w, ws, b = _operands(M, N, K, M + N + K)
+    want, bound = ref_product(x, xs, w, ws, b, False, dt)
+    torch.cuda.synchronize()
+    assert L.gcdr_k_status(None) == OK
+    for limit in (1, 3000, 30000, 1):
+        out, buf = strided(M, N, N + pad, dt, float("nan"))
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        assert i8_gemm(x, xs, w, ws, b, out, wait_cycles=limit) == 0
+        status = L.gcdr_k_status(None)
+        assert time.perf_counter() - t0 < 0.5, "waited for copies that nothing had issued"
+        assert status in (OK, 5)
+        done = ~torch.isnan(out)
+        assert status == 5 or done.all()
+        assert worst(torch.where(done, out.double(), want), want, bound) <= 1.0
+        assert torch.isnan(buf).sum() >= buf.numel() - M * N
+        assert L.gcdr_k_status(None) == OK
+    assert i8_gemm(x, xs, w, ws, b, out) == 0
+    assert worst(out, want, bound) <= 1.0
