@@ -633,25 +633,17 @@ __global__ void to_layout_kernel(const __half *src, int H, int W, int C, Act dst
 
 namespace {
 
-// One layer error word per device (the kernels' timeout flag of gcdr_k_conv), allocated and
-// zeroed on the device's first layer call; gcdr_k_status reads and clears it.
+// The current device's layer error word (the timeout flag of gcdr_k_conv's and gcdr_k_i8_gemm's kernels): a variable of
+// the library, so that nothing is allocated for it.  Its address is looked up on the device's first layer call;
+// gcdr_k_status reads and clears it.
 constexpr int kMaxLayerDevices = 64;
-std::mutex g_layer_err_mu;
-int *g_layer_err[kMaxLayerDevices] = {};
+std::atomic<int *> g_layer_err[kMaxLayerDevices];
 
 int *layer_err_word(int dev) {
     if (dev < 0 || dev >= kMaxLayerDevices) return nullptr;
-    std::lock_guard<std::mutex> lock(g_layer_err_mu);
-    if (!g_layer_err[dev]) {
-        int *p = nullptr;
-        if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-        if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) {
-            cudaFree(p);
-            return nullptr;
-        }
-        g_layer_err[dev] = p;
-    }
-    return g_layer_err[dev];
+    int *p = g_layer_err[dev].load(std::memory_order_acquire);
+    if (!p && (p = i8_error_word()) != nullptr) g_layer_err[dev].store(p, std::memory_order_release);
+    return p;
 }
 
 }  // namespace
@@ -689,7 +681,6 @@ extern "C" int gcdr_k_status(void *stream) {
     if (cudaMemcpy(&h, d_err, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess ||
         cudaMemset(d_err, 0, sizeof(int)) != cudaSuccess)
         return GCDR_ERR_DEVICE;
-    h |= i8_status_word();
     return (h & GCDR_ERR_FLAG_TIMEOUT) ? GCDR_ERR_TIMEOUT : h ? GCDR_ERR_DEVICE : GCDR_OK;
 }
 

@@ -1,5 +1,5 @@
 // int8.h -- the int8 token product (gcdr_k_i8_gemm): its arguments, its tensor-core kernel's launch, and the
-// status word that capi.cu reads.
+// layer error word that capi.cu reads.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -10,10 +10,8 @@
 
 namespace gcdr {
 
-constexpr int GCDR_ERR_FLAG_OTHER = 1 << 30;   // the status itself could not be read
-
-// Reads and clears the current device's error word of the int8 product (GCDR_ERR_FLAG_*).
-int i8_status_word();
+// The current device's layer error word, which the int8 product's kernels set (null: it cannot be had).
+int *i8_error_word();
 
 struct I8Args {
     int64_t M;

@@ -35,7 +35,7 @@
 namespace gcdr {
 namespace {
 
-__device__ int g_i8_err;   // set by a kernel whose bounded wait ran out (GCDR_ERR_FLAG_*)
+__device__ int g_i8_err;   // the device's layer error word (GCDR_ERR_FLAG_*): a kernel's bounded wait ran out
 
 constexpr int kFirstEpi = 4;
 constexpr int kBlockK = 128;                       // bytes of K per ring stage (one 128-byte swizzle row)
@@ -809,15 +809,11 @@ void i8_tc_form(const I8Args &a, int sms, gcdr_i8_form &f) {
     f.units = (int64_t)pl.tiles_p * pl.tiles_q;
 }
 
-int i8_status_word() {
-    int h = 0;
-    const int zero = 0;
-    if (cudaMemcpyFromSymbol(&h, g_i8_err, sizeof h) != cudaSuccess ||
-        (h && cudaMemcpyToSymbol(g_i8_err, &zero, sizeof zero) != cudaSuccess)) {
-        cudaGetLastError();
-        return GCDR_ERR_FLAG_OTHER;
-    }
-    return h;
+int *i8_error_word() {
+    void *p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_i8_err) == cudaSuccess) return static_cast<int *>(p);
+    cudaGetLastError();
+    return nullptr;
 }
 
 }  // namespace gcdr
