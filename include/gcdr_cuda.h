@@ -365,10 +365,22 @@ GCDR_API int gcdr_k_conv_static(const gcdr_conv_desc *d, void *stream);
  *
  * The token products of an int8 deployment and what surrounds them, beside the fp16 token
  * Gemm (gcdr_k_conv kind 2) and its LayerNorm finalize.  No counterpart in the reference (its
- * engines run fp32).  A chain of them, as one block uses it:
+ * engines run fp32).
  *
- *   gcdr_k_block_norm  (norm; rows out as int8)  ->  gcdr_k_i8_gemm  ->  gcdr_k_dw_gelu_shift
- *   ->  gcdr_k_quant_rows  ->  gcdr_k_i8_gemm  ->  gcdr_k_block_norm  (post-norm, gate, residual)
+ * The models' shifted-MLP block moves channel groups between tokens (the shift along H) between its
+ * norm and its first product.  A token's scale is that of its shifted row, so its rows are rounded behind
+ * the entry that shifts:
+ *
+ *   gcdr_k_ln_finalize or gcdr_k_up_add (norm, H shift)  ->  gcdr_k_quant_rows  ->  gcdr_k_i8_gemm (fc1)
+ *   ->  gcdr_k_dw_gelu_shift  ->  gcdr_k_quant_rows  ->  gcdr_k_i8_gemm (fc2: fp32, no bias)
+ *   ->  gcdr_k_ln_finalize (ksplit 1: bias, residual, norm, and the next norm with its H shift)
+ *
+ * (error of such a block against the fp32 block: 0.003 to 0.006 rms at an output of 1 rms).
+ * gcdr_k_block_norm has no shift and takes no part in that block.  It serves blocks whose products follow
+ * their norms directly (RMS norms, gates, a residual scale, C beyond 512):
+ *
+ *   gcdr_k_block_norm (norm; rows out as int8)  ->  gcdr_k_i8_gemm  ->  the block's middle  ->
+ *   gcdr_k_quant_rows  ->  gcdr_k_i8_gemm  ->  gcdr_k_block_norm (post-norm, gate, residual, next norm)
  *
  * Common to the three.  All pointers are DEVICE pointers of the current device (anything
  * else is GCDR_ERR_ARG); calls only enqueue work on `stream` (NULL = default stream), allocate
