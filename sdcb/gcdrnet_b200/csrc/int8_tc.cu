@@ -648,8 +648,10 @@ uintptr_t result_place(const I8Args &a) {   // what the starts of the result's r
     return reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * dtype_bytes(a.dtype));
 }
 
-// Picks form and tile by an estimate in SM cycles, fitted to measured sweeps (B200, K 256 to 8192, 16 to 57600
-// tokens, 160 to 8192 channels; within 15 % of the best form there):
+// Picks form and tile by an estimate in SM cycles, fitted to measured sweeps on a B200.  Against every form forced in turn:
+// 93 % of random sizes are within 15 % of the best one (K 256 to 8192, 16 to 57600 tokens, 160 to 8192 channels; and as many
+// of smaller K and N), the worst 2.1 times (2.5) as slow: splits of four at 34 to 37 units, which take a second round
+// (33 clusters of four fit 148 SMs), and 260 to 512 tokens with K up to 300 against thousands of channels.
 //   a k-block step     what its loads and MMAs take together (a pair's for twice the rows; the second figures where
 //                      rows do not start on a line: each 128 bytes are then two requests); 16 epilogue warps leave a
 //                      ring stage less
@@ -657,7 +659,7 @@ uintptr_t result_place(const I8Args &a) {   // what the starts of the result's r
 //                      at multiples of 8 bytes only 10 (a pair 8) and 13, at any element 8 (6) and 11
 //   a round            700 between units; the last one's results and the start are not hidden (nor, of two units, the
 //                      second half of the warps)
-//   a split of K       the join's words through distributed shared memory; clusters of eight fit the GPU 12 times
+//   a split of K       the join's words through distributed shared memory; clusters of eight fit 148 SMs 12 times
 // E.g. 57600 x 256 x 256 fp16: wide 128, 16 warps 11.7 us, 8 warps 14.5, wide 256 13.0; 1213 x 1040 x 1000 fp32: wide 128
 // 7.4 us, 64 8.8, 256 10.5; 128 x 8192 x 8192: wide 64 16.9 us, 128 20.1; 4096^3: pair 48 us, wide 256 53, 128 56;
 // 128 x 1024 x 8192: narrow 32 split 4 9.0 us, wide 64 11.1; 16 x 1024 x 8192: split 8 6.4 us, 4 7.1, 2 9.3, none 11.3.

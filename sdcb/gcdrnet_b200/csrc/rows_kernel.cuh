@@ -4,9 +4,9 @@
 //   block_norm   v = x + res_scale * gate . N1(f);  r = v;  h = N2(v) as y or as int8 rows
 //                N = LayerNorm (u - mean) / sqrt(var + eps) * g + b, or RMS u / sqrt(mean u^2 + eps) * g + b
 //
-// Both are bound by memory: each element is read once into registers, every statistic is taken there in
-// fp32 (the mean first, then the squares about it), and the row is written once.  v stays in fp32 for the
-// second norm: only what is stored is rounded to the activations' type.
+// Both are bound by memory: each element is read once into registers (rows too long for them: see rows_launch), every
+// statistic is taken there in fp32 (the mean first, then the squares about it), and the row is written once.  v stays in
+// fp32 for the second norm: only what is stored is rounded to the activations' type.
 //
 // A group of G threads holds a row, 8 * NCH elements a thread, and walks the rows with the resident blocks of the
 // whole GPU; an operand's next row is on its way as soon as this one's registers are free.
@@ -134,7 +134,7 @@ __device__ __forceinline__ float inv_sqrt(float a) {
 // rows are not aligned, pairs or single ones G apart.  `raw` keeps them as they lie in memory.  Pointers are those of the
 // thread's first element, `left` what the row has from there on.
 // FIT: kOdd rows start anywhere, kPair rows are whole pairs of elements (8192 x 2046 fp16, both LayerNorm and a gate: 33 us
-// against 44 by single elements; to int8 9.9 and 13.1; fp32 norm 55 and 57), kVec rows whole 16-byte pieces, kFull rows
+// against 44 by single elements; to int8 9.9 and 13.1; fp32 norm 51 and 53), kVec rows whole 16-byte pieces, kFull rows
 // too and fill their group (nothing lies past the end).
 enum Fit : int { kOdd, kPair, kVec, kFull };
 template <class T, int G, int NCH, Fit FIT>
@@ -483,6 +483,10 @@ cudaError_t launch_rows(const RowArgs &a, int piece, cudaStream_t st) {
 // 256 x 32 107, 512 x 16 143; 16384 of 2048 64 x 32 48, 128 x 16 54); shorter rows, fp32 rows and the rounding alone do
 // not (1024 bf16 64 x 16 51 us, 32 x 32 50, RMS 46 and 49; 8192 to int8 512 x 16 40, 256 x 32 45).  Beyond 8192 the
 // registers of larger blocks decide (4096 rows of 16384 bf16, RMS: 512 x 32 97 us, 1024 x 16 147; to int8 46 and 41).
+// Past 8192 elements in fp32, and past 12288 (odd places) or 16384 in 16 bits, these blocks' registers do not hold a row beside
+// the next one's operands: part of them lies in local memory (fp32 norms 60 bytes a thread up to 12288 elements, 0.4 KB up to
+// 16384, 1.7 to 4.2 KB at 32768; both LayerNorm with a gate, over the floor of their bytes: fp32 12288 1.2, 16384 1.6, 24576
+// 2.9, 32768 7.3 times; fp16 16384 1.5, 24576 2.4, 32768 2.9).
 template <class T, bool QUANT>
 cudaError_t rows_launch(const RowArgs &a, int piece, cudaStream_t st) {
     const auto fits = [&](int g, int nch) { return a.C <= 8 * g * nch; };
