@@ -390,7 +390,12 @@ GCDR_API int gcdr_k_conv_static(const gcdr_conv_desc *d, void *stream);
  * rows: GCDR_OK, nothing is launched.  A refused call prints the reason to stderr and launches
  * nothing: GCDR_ERR_ARG (null, unaligned, overlapping or foreign operands, unknown codes), GCDR_ERR_RANGE
  * (sizes and pitches).  The same call gives the same bytes, whatever runs beside it, and a row's
- * bytes do not depend on the call's other rows (at the same alignment). */
+ * bytes do not depend on the call's other rows (at the same alignment).
+ *
+ * Every operand may be an output of the call before on the stream.  (gcdr_k_conv, gcdr_k_dw_gelu_shift and
+ * gcdr_k_ln_finalize take weights and biases for constants and may read them while earlier calls of this
+ * library still run: one that such a call computes needs a wait, or a copy or kernel of the caller's own, in
+ * between.) */
 #define GCDR_DTYPE_F16 0
 #define GCDR_DTYPE_BF16 1
 #define GCDR_DTYPE_F32 2
@@ -407,6 +412,7 @@ GCDR_API int gcdr_k_quant_rows(const void *x, int dtype, int64_t rows, int C, in
 
 /* out[m][n] = xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n], then relu (a NaN stays NaN, a zero has no
  * sign), rounded to `dtype`.  The integer sum is exact: K 1..131071 (int32 sums of products up to 2^14).
+ * It is converted to fp32 and takes xs[m], then ws[n]: the sum times xs[m] has to fit fp32's normal numbers.
  *   x    int8 [M][K], pitch ldx, xs M scales;   w  int8 [N][K], pitch ldw, ws N scales
  *        x and w 16-byte aligned, ldx and ldw multiples of 16 (K and N are free); rows on
  *        128-byte lines (ldx, ldw multiples of 128) read up to twice as fast
